@@ -1,0 +1,1021 @@
+// ddt_classes.hip -- operators on a matrix of class scores (row r, class c): adjust (penalties for repeated classes, biases, masks),
+// top (the k best classes of each row and the row's log-sum-exp), distill (a student's loss against a teacher's top scores, and its
+// gradient).  All of them read the matrix once from HBM and do little per score: bandwidth is what bounds them.
+//
+// A 16-byte piece of a row is a "pack" (4 fp32 or 8 two-byte scores).  Rows start at any address (an odd number of classes): global
+// memory takes a 16-byte access at any element address, so packs count from the row's own start and only a row's last pack is partial.
+// Arithmetic is fp32 or wider whatever the scores' type; a result is rounded once, to nearest even, when it is stored.
+#include <hip/hip_runtime.h>
+#include <float.h>
+#include <math.h>
+
+#include "../../include/ddt.h"
+#include "ddt_classes.h"
+
+namespace ddt {
+namespace {
+
+extern __shared__ uint32_t lds_words[];
+
+constexpr float kInf = __builtin_inff();
+
+template <class T>
+struct Pack {
+  static constexpr uint32_t N = 16 / sizeof(T);
+  typedef T vec __attribute__((ext_vector_type(16 / sizeof(T))));
+};
+
+// scores [c, c + N) of a row of `end` classes; `fill` behind its end
+template <class T>
+__device__ __forceinline__ void load_pack(const T* row, uint32_t c, uint32_t end, float fill, float (&x)[Pack<T>::N]) {
+  constexpr uint32_t N = Pack<T>::N;
+  if (c + N <= end) {
+    typename Pack<T>::vec v;
+    __builtin_memcpy(&v, row + c, 16);
+#pragma unroll
+    for (uint32_t i = 0; i < N; ++i) x[i] = (float)v[i];
+  } else {
+#pragma unroll
+    for (uint32_t i = 0; i < N; ++i) x[i] = c + i < end ? (float)row[c + i] : fill;
+  }
+}
+template <class T>
+__device__ __forceinline__ void store_pack(T* row, uint32_t c, uint32_t end, const float (&x)[Pack<T>::N]) {
+  constexpr uint32_t N = Pack<T>::N;
+  if (c + N <= end) {
+    typename Pack<T>::vec v;
+#pragma unroll
+    for (uint32_t i = 0; i < N; ++i) v[i] = (T)x[i];
+    __builtin_memcpy(row + c, &v, 16);
+  } else {
+#pragma unroll
+    for (uint32_t i = 0; i < N; ++i)
+      if (c + i < end) row[c + i] = (T)x[i];
+  }
+}
+
+// x ^ 2: the hardware instruction (1 ulp; results below 2^-126 may come back as 0 -- nothing next to a sum whose largest term is 1)
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// ---------------------------------------------------------------------------------------------------
+// adjust
+// ---------------------------------------------------------------------------------------------------
+// word of the history counter: times the class stands behind the row's prompt part, bit 31 = it stands in the prompt part
+constexpr uint32_t kInPrompt = 0x80000000u;
+
+struct RowPenalty {
+  float rep, freq, pres;
+};
+__device__ __forceinline__ RowPenalty row_penalty(const AdjustArgs& a, uint64_t r) {
+  return {a.repetition ? a.repetition[r] : 1.f, a.frequency ? a.frequency[r] : 0.f, a.presence ? a.presence[r] : 0.f};
+}
+__device__ __forceinline__ float penalise(float x, uint32_t w, const RowPenalty& p) {
+  if (w == 0u) return x;
+  x = x > 0.f ? x / p.rep : x * p.rep;
+  const uint32_t behind = w & ~kInPrompt;
+  x = x - p.freq * (float)behind;
+  return behind ? x - p.pres : x;
+}
+
+// counts the history of rows [r0, r0 + rows) for classes [c0, c0 + C) into counts[r * row_pitch + c * class_pitch] (zeroed, synchronised).
+// Integer LDS adds: their order does not show.  Offsets and class numbers come from the device unchecked: offsets are clamped to the
+// history's length, numbers outside the tile (also outside the matrix) count nowhere.
+__device__ __forceinline__ void count_history(const AdjustArgs& a, uint64_t r0, uint32_t rows, uint32_t c0, uint32_t C, uint32_t row_pitch,
+                                              uint32_t class_pitch, uint32_t* counts) {
+  const uint32_t waves = blockDim.x >> 6;
+  const bool per_wave = rows >= waves;  // a wave per row; fewer rows than waves: all threads on one row after the other
+  const uint32_t step = per_wave ? 64u : blockDim.x, lane = per_wave ? threadIdx.x & 63u : threadIdx.x;
+  for (uint32_t r = per_wave ? threadIdx.x >> 6 : 0u; r < rows; r += per_wave ? waves : 1u) {
+    const int64_t len = (int64_t)a.history_len;
+    int64_t lo = a.first[r0 + r], hi = a.first[r0 + r + 1];
+    lo = lo < 0 ? 0 : lo > len ? len : lo;
+    hi = hi < lo ? lo : hi > len ? len : hi;
+    int64_t split = a.prompt ? (int64_t)a.prompt[r0 + r] : 0;
+    split = split < 0 ? lo : split > hi - lo ? hi : lo + split;
+    uint32_t* row = counts + r * row_pitch;
+    for (int64_t i = lo + lane; i < hi; i += step) {
+      const uint32_t c = (uint32_t)a.history[i] - c0;
+      if (c < C) {
+        if (i >= split) atomicAdd(&row[c * class_pitch], 1u);
+        else atomicOr(&row[c * class_pitch], kInPrompt);
+      }
+    }
+  }
+}
+
+struct AdjustTiles {
+  uint32_t rows, classes;      // of a tile; row-major: classes is a multiple of the pack
+  uint32_t magic;              // row-major: idx / (classes / N) = umulhi(idx, magic)
+  uint64_t class_tiles, tiles;
+};
+
+template <class T, bool HIST>
+__global__ __launch_bounds__(256) void adjust_rows_kernel(const AdjustArgs a, const AdjustTiles t) {
+  constexpr uint32_t N = Pack<T>::N;
+  const uint32_t ppr = t.classes / N;
+  for (uint64_t tile = blockIdx.x; tile < t.tiles; tile += gridDim.x) {
+    const uint64_t rt = tile / t.class_tiles, r0 = rt * t.rows;
+    const uint32_t c0 = (uint32_t)(tile - rt * t.class_tiles) * t.classes;
+    const uint32_t rows = (uint32_t)(a.n - r0 < t.rows ? a.n - r0 : t.rows);
+    const uint32_t C = a.K - c0 < t.classes ? a.K - c0 : t.classes;
+    if (HIST) {
+      __syncthreads();  // the tile before has been read
+      for (uint32_t i = threadIdx.x; i < rows * t.classes; i += 256u) lds_words[i] = 0u;
+      __syncthreads();
+      count_history(a, r0, rows, c0, C, t.classes, 1u, lds_words);
+      __syncthreads();
+    }
+    for (uint32_t idx = threadIdx.x; idx < rows * ppr; idx += 256u) {
+      const uint32_t q = t.rows == 1u ? 0u : ppr == 1u ? idx : __umulhi(idx, t.magic), cl = (idx - q * ppr) * N, c = c0 + cl;
+      if (cl >= C) continue;
+      const uint64_t r = r0 + q;
+      float x[N];
+      load_pack(static_cast<const T*>(a.in) + r * a.in_stride, c, a.K, 0.f, x);
+      if (HIST) {
+        uint32_t w[N], any = 0u;
+#pragma unroll
+        for (uint32_t i = 0; i < N; ++i) any |= w[i] = lds_words[q * t.classes + cl + i];
+        if (any) {
+          const RowPenalty p = row_penalty(a, r);
+#pragma unroll
+          for (uint32_t i = 0; i < N; ++i) x[i] = penalise(x[i], w[i], p);
+        }
+      }
+      if (a.bias) {
+        const float* b = a.bias + r * a.bias_rs;
+        if (a.bias_cs == 1u && c + N <= a.K) {
+#pragma unroll
+          for (uint32_t i = 0; i < N; i += 4) {
+            Pack<float>::vec v;
+            __builtin_memcpy(&v, b + c + i, 16);
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) x[i + j] += v[j];
+          }
+        } else {
+#pragma unroll
+          for (uint32_t i = 0; i < N; ++i)
+            if (c + i < a.K) x[i] += b[(uint64_t)(c + i) * a.bias_cs];
+        }
+      }
+      if (a.allowed) {  // a pack's bits stand in one word
+        const uint32_t bits = a.allowed[r * a.allowed_rs + (c >> 5)] >> (c & 31u);
+#pragma unroll
+        for (uint32_t i = 0; i < N; ++i) x[i] = (bits >> i) & 1u ? x[i] : -kInf;
+      }
+      store_pack(static_cast<T*>(a.out) + r * a.out_stride, c, a.K, x);
+    }
+  }
+}
+
+// class-major: packs run along the rows of one class; a tile's packs per class are a power of two
+template <class T, bool HIST>
+__global__ __launch_bounds__(256) void adjust_classes_kernel(const AdjustArgs a, const AdjustTiles t) {
+  constexpr uint32_t N = Pack<T>::N;
+  const uint32_t rp = t.rows / N, rp_log2 = 31u - __clz(rp);
+  for (uint64_t tile = blockIdx.x; tile < t.tiles; tile += gridDim.x) {
+    const uint64_t rt = tile / t.class_tiles, r0 = rt * t.rows;
+    const uint32_t c0 = (uint32_t)(tile - rt * t.class_tiles) * t.classes;
+    const uint32_t rows = (uint32_t)(a.n - r0 < t.rows ? a.n - r0 : t.rows);
+    const uint32_t C = a.K - c0 < t.classes ? a.K - c0 : t.classes;
+    if (HIST) {
+      __syncthreads();
+      for (uint32_t i = threadIdx.x; i < C * t.rows; i += 256u) lds_words[i] = 0u;
+      __syncthreads();
+      count_history(a, r0, rows, c0, C, 1u, t.rows, lds_words);
+      __syncthreads();
+    }
+    for (uint32_t idx = threadIdx.x; idx < (C << rp_log2); idx += 256u) {
+      const uint32_t cl = idx >> rp_log2, rl = (idx & (rp - 1u)) * N, c = c0 + cl;
+      if (rl >= rows) continue;
+      float x[N];
+      load_pack(static_cast<const T*>(a.in) + c * a.in_stride + r0, rl, rows, 0.f, x);
+      if (HIST) {
+        uint32_t w[N], any = 0u;
+#pragma unroll
+        for (uint32_t i = 0; i < N; ++i) any |= w[i] = lds_words[cl * t.rows + rl + i];
+        if (any) {
+#pragma unroll
+          for (uint32_t i = 0; i < N; ++i)
+            if (w[i]) x[i] = penalise(x[i], w[i], row_penalty(a, r0 + rl + i));
+        }
+      }
+      if (a.bias) {
+        const float* b = a.bias + (uint64_t)c * a.bias_cs;
+        if (a.bias_rs == 0u) {
+          const float v = b[0];
+#pragma unroll
+          for (uint32_t i = 0; i < N; ++i) x[i] += v;
+        } else {
+#pragma unroll
+          for (uint32_t i = 0; i < N; ++i)
+            if (rl + i < rows) x[i] += b[(r0 + rl + i) * a.bias_rs];
+        }
+      }
+      if (a.allowed) {
+        const uint32_t* m = a.allowed + (c >> 5);
+        if (a.allowed_rs == 0u) {
+          const bool on = (m[0] >> (c & 31u)) & 1u;
+#pragma unroll
+          for (uint32_t i = 0; i < N; ++i) x[i] = on ? x[i] : -kInf;
+        } else {
+#pragma unroll
+          for (uint32_t i = 0; i < N; ++i)
+            if (rl + i < rows) x[i] = (m[(r0 + rl + i) * a.allowed_rs] >> (c & 31u)) & 1u ? x[i] : -kInf;
+        }
+      }
+      store_pack(static_cast<T*>(a.out) + c * a.out_stride + r0, rl, rows, x);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------
+// sums of exponentials: (m, s) = (largest score so far, sum of exp((x - m) / T)).  The difference is taken before the scaling: it is
+// finite for finite scores (a row filled with the type's lowest value among them), and small, so exact enough, where it counts.
+// ---------------------------------------------------------------------------------------------------
+struct ExpSum {
+  float m = -FLT_MAX, s = 0.f;
+  template <uint32_t N>
+  __device__ __forceinline__ void add(const float (&x)[N], float c) {
+    float pm = x[0];
+#pragma unroll
+    for (uint32_t i = 1; i < N; ++i) pm = fmaxf(pm, x[i]);
+    if (pm > m) {
+      s *= exp2_fast((m - pm) * c);
+      m = pm;
+    }
+    float t = 0.f;
+#pragma unroll
+    for (uint32_t i = 0; i < N; ++i) t += exp2_fast((x[i] - m) * c);
+    s += t;
+  }
+  __device__ __forceinline__ void merge(float om, float os, float c) {
+    const float M = fmaxf(m, om);
+    s = s * exp2_fast((m - M) * c) + os * exp2_fast((om - M) * c);
+    m = M;
+  }
+  __device__ __forceinline__ void reduce_wave(float c) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) merge(__shfl_xor(m, d), __shfl_xor(s, d), c);
+  }
+};
+__device__ __forceinline__ float log_sum(const ExpSum& e, double inv_T) {
+  if (e.m == kInf) return kInf;
+  return (float)((double)e.m * inv_T + log((double)e.s));  // nothing but -inf: log 0 = -inf
+}
+
+// ---------------------------------------------------------------------------------------------------
+// top: whole numbers in the order of the scores; 0 = no candidate (NaN, -inf).  -0 and +0 are one score.
+// ---------------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t score_key(float x) {
+  const uint32_t b = __float_as_uint(x + 0.f);
+  return x > -kInf ? b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u) : 0u;
+}
+__device__ __forceinline__ float key_score(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
+// low key bits that are alike for every score of a sign (two-byte types): they need no search
+template <class T>
+constexpr uint32_t low_bits() {
+  return sizeof(T) == 4 ? 0u : __is_same(T, _Float16) ? 13u : 16u;
+}
+// (key, class) in one number: the larger is the better candidate, equal scores go to the lower class
+__device__ __forceinline__ uint64_t candidate(uint32_t key, uint32_t c) { return (uint64_t)key << 32 | (0xFFFFFFFFu - c); }
+
+__device__ __forceinline__ void write_candidate(const TopArgs& a, uint64_t row, uint32_t rank, uint64_t v) {
+  a.ids[row * a.k + rank] = (int32_t)(0xFFFFFFFFu - (uint32_t)v);
+  a.values[row * a.k + rank] = key_score((uint32_t)(v >> 32));
+}
+__device__ __forceinline__ void write_nothing(const TopArgs& a, uint64_t row, uint32_t rank) {
+  a.ids[row * a.k + rank] = -1;
+  a.values[row * a.k + rank] = -kInf;
+}
+
+// few classes, few of them wanted: a thread per row, the best KK in registers.  Row-major rows are staged in LDS (coalesced loads;
+// the row pitch is an odd number of words), class-major ones are coalesced as they are.
+template <class T>
+__device__ __forceinline__ uint32_t staged_pitch(uint32_t K) {  // elements
+  constexpr uint32_t per_word = 4 / sizeof(T);
+  return (((K + per_word - 1) / per_word) | 1u) * per_word;
+}
+template <class T>
+__device__ __forceinline__ void stage_rows(const T* in, uint64_t r0, uint32_t rows, uint32_t K, uint64_t stride, T* dst, uint32_t pitch) {
+  if (stride == K) {  // one piece of rows * K scores (at most 256 * 32)
+    const T* src = in + r0 * K;
+    const uint32_t total = rows * K, magic = (uint32_t)((0x100000000ull + K - 1u) / K);  // K >= 2: i / K = umulhi(i, magic) for i < 2^16
+    constexpr uint32_t N = Pack<T>::N;
+    for (uint32_t i = threadIdx.x * N; i < total; i += 256u * N) {
+      uint32_t r = K == 1u ? i : __umulhi(i, magic), c = i - r * K;
+      typename Pack<T>::vec v;
+      if (i + N <= total) __builtin_memcpy(&v, src + i, 16);
+      else {
+#pragma unroll
+        for (uint32_t j = 0; j < N; ++j) v[j] = i + j < total ? src[i + j] : (T)0.f;
+      }
+#pragma unroll
+      for (uint32_t j = 0; j < N; ++j) {
+        if (i + j < total) dst[r * pitch + c] = v[j];
+        if (++c == K) c = 0u, ++r;
+      }
+    }
+  } else {
+    for (uint32_t r = threadIdx.x >> 5; r < rows; r += 8u)
+      for (uint32_t c = threadIdx.x & 31u; c < K; c += 32u) dst[r * pitch + c] = in[(r0 + r) * stride + c];
+  }
+}
+
+template <class T, bool CM, int KK>
+__global__ __launch_bounds__(256) void top_thread_kernel(const TopArgs a) {
+  T* stage = reinterpret_cast<T*>(lds_words);
+  const uint32_t pitch = staged_pitch<T>(a.K);
+  const float c2 = (float)(1.4426950408889634 / a.temperature);
+  const uint64_t step = (uint64_t)gridDim.x * 256u;
+  for (uint64_t r0 = (uint64_t)blockIdx.x * 256u; r0 < a.n; r0 += step) {
+    const uint32_t rows = (uint32_t)(a.n - r0 < 256u ? a.n - r0 : 256u);
+    const T* in = static_cast<const T*>(a.in);
+    if (!CM) {
+      __syncthreads();
+      stage_rows(in, r0, rows, a.K, a.stride, stage, pitch);
+      __syncthreads();
+    }
+    if (threadIdx.x >= rows) continue;
+    const uint64_t row = r0 + threadIdx.x;
+    float v[KK];
+    int32_t id[KK];
+#pragma unroll
+    for (int j = 0; j < KK; ++j) v[j] = -kInf, id[j] = -1;
+    ExpSum e;
+    for (uint32_t c = 0; c < a.K; ++c) {
+      const float x1[1] = {(float)(CM ? in[c * a.stride + row] : stage[threadIdx.x * pitch + c])};
+      e.add(x1, c2);
+      float x = x1[0];
+      if (x > v[KK - 1]) {  // (false for NaN and -inf)
+        int32_t xi = (int32_t)c;
+        bool placed = false;
+#pragma unroll
+        for (int j = 0; j < KK; ++j) {  // equal scores: the class that came first stays in front
+          placed |= x > v[j];
+          const float tv = v[j];
+          const int32_t ti = id[j];
+          v[j] = placed ? x : tv, id[j] = placed ? xi : ti;
+          x = placed ? tv : x, xi = placed ? ti : xi;
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < KK; ++j)
+      if ((uint32_t)j < a.k) a.ids[row * a.k + j] = id[j], a.values[row * a.k + j] = v[j];
+    if (a.lse) a.lse[row] = log_sum(e, 1.0 / a.temperature);
+  }
+}
+
+// the kk-th largest of the keys in a wave's registers (E per lane): greedy from the top bit, counted with ballots
+template <int E>
+__device__ __forceinline__ uint32_t wave_kth_key(const uint32_t (&key)[E], uint32_t kk, uint32_t low) {
+  uint32_t t = 0u;
+  for (int bit = 31; bit >= (int)low; --bit) {
+    const uint32_t cand = t | (1u << bit);
+    uint32_t cnt = 0u;
+#pragma unroll
+    for (int i = 0; i < E; ++i) cnt += __popcll(__ballot(key[i] >= cand));
+    if (cnt >= kk) {
+      t = cand;
+      if (cnt == kk) break;  // exactly the kk best: a lower bound that admits no others
+    }
+  }
+  return t;
+}
+
+// up to 2048 classes: a wave per row, all its keys in registers (P packs per lane).  Class-major rows are staged through LDS, 16 at a
+// time (64-byte pieces of fp32), for the 8 waves of the block.
+constexpr uint32_t top_wave_rows(bool class_major) { return class_major ? 16u : 4u; }
+constexpr uint32_t top_wave_waves(bool class_major) { return class_major ? 8u : 4u; }
+template <class T, bool CM, int P>
+__global__ __launch_bounds__(top_wave_waves(CM) * 64) void top_wave_kernel(const TopArgs a) {
+  constexpr int N = (int)Pack<T>::N, E = P * N;
+  constexpr uint32_t kRows = top_wave_rows(CM), kWaves = top_wave_waves(CM);
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+  uint64_t* list = reinterpret_cast<uint64_t*>(lds_words) + wave * a.k;  // the wave's selected candidates
+  T* stage = reinterpret_cast<T*>(reinterpret_cast<uint64_t*>(lds_words) + kWaves * a.k);  // class-major: [K][16] scores
+  const float c2 = (float)(1.4426950408889634 / a.temperature);
+  for (uint64_t r0 = (uint64_t)blockIdx.x * kRows; r0 < a.n; r0 += (uint64_t)gridDim.x * kRows) {
+    if (CM) {
+      __syncthreads();
+      const uint32_t r = threadIdx.x & 15u;
+      if (r0 + r < a.n)
+        for (uint32_t c = threadIdx.x >> 4; c < a.K; c += kWaves * 4u) stage[c * 16u + r] = static_cast<const T*>(a.in)[c * a.stride + r0 + r];
+      __syncthreads();
+    }
+    for (uint32_t rr = wave; rr < kRows && r0 + rr < a.n; rr += kWaves) {
+      const uint64_t row = r0 + rr;
+      uint32_t key[E];
+      ExpSum e;
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        const uint32_t c = ((uint32_t)p * 64u + lane) * N;
+        float x[N];
+        if (CM) {
+#pragma unroll
+          for (int i = 0; i < N; ++i) x[i] = c + i < a.K ? (float)stage[(c + i) * 16u + rr] : -kInf;
+        } else {
+          load_pack(static_cast<const T*>(a.in) + row * a.stride, c, a.K, -kInf, x);
+        }
+        e.add(x, c2);
+#pragma unroll
+        for (int i = 0; i < N; ++i) key[p * N + i] = score_key(x[i]);
+      }
+      e.reduce_wave(c2);
+      if (a.lse && lane == 0u) a.lse[row] = log_sum(e, 1.0 / a.temperature);
+      uint32_t valid = 0u;
+#pragma unroll
+      for (int i = 0; i < E; ++i) valid += __popcll(__ballot(key[i] != 0u));
+      const uint32_t kk = valid < a.k ? valid : a.k;
+      uint32_t t = wave_kth_key(key, kk, low_bits<T>());
+      if (t == 0u) t = 1u;  // (fewer than k candidates: all of them)
+      // everything from t up, if that is kk; else what lies above t's score, and of the classes with t's score the lowest ones
+      uint32_t ge = 0u, gt = 0u;
+      const uint32_t above = t + (1u << low_bits<T>());
+#pragma unroll
+      for (int i = 0; i < E; ++i) ge += __popcll(__ballot(key[i] >= t)), gt += __popcll(__ballot(key[i] >= above));
+      uint32_t last = 0xFFFFFFFFu;  // highest class admitted among the equal ones
+      if (ge > kk) {
+        last = 0u;
+        for (int bit = 10; bit >= 0; --bit) {  // (at most 2048 classes)
+          const uint32_t cand = last + (1u << bit);
+          uint32_t cnt = gt;
+#pragma unroll
+          for (int i = 0; i < E; ++i) {
+            const uint32_t c = ((uint32_t)(i / N) * 64u + lane) * N + i % N;
+            cnt += __popcll(__ballot(key[i] >= t && key[i] < above && c < cand));
+          }
+          if (cnt < kk) last = cand;
+        }
+      }
+      uint32_t base = 0u;
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        const uint32_t c = ((uint32_t)(i / N) * 64u + lane) * N + i % N;
+        const bool take = key[i] >= t && (key[i] >= above || c <= last);
+        const uint64_t b = __ballot(take);
+        if (take) list[base + __popcll(b & ((1ull << lane) - 1ull))] = candidate(key[i], c);
+        base += __popcll(b);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      for (uint32_t i = lane; i < a.k; i += 64u) {
+        if (i >= base) {
+          write_nothing(a, row, i);
+          continue;
+        }
+        const uint64_t mine = list[i];
+        uint32_t rank = 0u;
+        for (uint32_t j = 0; j < base; ++j) rank += list[j] > mine;
+        write_candidate(a, row, rank, mine);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();  // the next row's candidates go into the same list
+    }
+  }
+}
+
+// many classes: a block of NT threads per row.  One pass keeps each thread's largest score and its sum of exponentials; the k-th largest
+// of the NT maxima is a bound that at least k scores reach, and only the threads whose maximum reaches it -- about k of them -- read
+// their scores a second time to list the candidates.  Rows with more candidates than the list holds (scores that tie, or stand in few
+// threads) are narrowed down by counting, bit by bit, over the threads that reach the bound.
+constexpr uint32_t kListCap = 1024;
+template <class T, int NT>
+__global__ __launch_bounds__(NT) void top_block_kernel(const TopArgs a) {
+  constexpr uint32_t N = Pack<T>::N, kWaves = NT / 64;
+  uint64_t* list = reinterpret_cast<uint64_t*>(lds_words);         // [kListCap]
+  uint32_t* maxima = lds_words + 2 * kListCap;                     // [NT]
+  float* part = reinterpret_cast<float*>(maxima + NT);             // [2 * kWaves]
+  uint32_t* ctl = reinterpret_cast<uint32_t*>(part + 2 * kWaves);  // [0] bound, [1] candidates, [2 ..] counts per wave
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
+  const uint32_t packs = (a.K + N - 1u) / N;
+  const float c2 = (float)(1.4426950408889634 / a.temperature);
+  for (uint64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
+    const T* in = static_cast<const T*>(a.in) + row * a.stride;
+    ExpSum e;
+    float top = -kInf;
+    for (uint32_t p = tid; p < packs; p += NT) {
+      float x[N];
+      load_pack(in, p * N, a.K, -kInf, x);
+      e.add(x, c2);
+#pragma unroll
+      for (uint32_t i = 0; i < N; ++i) top = fmaxf(top, x[i]);
+    }
+    const uint32_t best = score_key(top);
+    e.reduce_wave(c2);
+    __syncthreads();  // the row before is written
+    maxima[tid] = best;
+    if (lane == 0u) part[2 * wave] = e.m, part[2 * wave + 1] = e.s;
+    if (tid == 0u) ctl[1] = 0u;
+    __syncthreads();
+    if (wave == 0u) {
+      constexpr int E = NT / 64;
+      uint32_t key[E];
+#pragma unroll
+      for (int i = 0; i < E; ++i) key[i] = maxima[i * 64 + lane];
+      const uint32_t t = wave_kth_key(key, a.k, low_bits<T>());
+      if (lane == 0u) ctl[0] = t ? t : 1u;
+    } else if (wave == 1u && a.lse) {
+      ExpSum w;
+      w.m = lane < kWaves ? part[2 * lane] : -FLT_MAX, w.s = lane < kWaves ? part[2 * lane + 1] : 0.f;
+      w.reduce_wave(c2);
+      if (lane == 0u) a.lse[row] = log_sum(w, 1.0 / a.temperature);
+    }
+    __syncthreads();
+    const uint32_t bound = ctl[0];
+    const bool mine = best >= bound;
+    if (mine)
+      for (uint32_t p = tid; p < packs; p += NT) {
+        float x[N];
+        load_pack(in, p * N, a.K, -kInf, x);
+#pragma unroll
+        for (uint32_t i = 0; i < N; ++i) {
+          const uint32_t key = score_key(x[i]);
+          if (key >= bound) {
+            const uint32_t slot = atomicAdd(&ctl[1], 1u);
+            if (slot < kListCap) list[slot] = candidate(key, p * N + i);
+          }
+        }
+      }
+    __syncthreads();
+    uint32_t count = ctl[1];
+    if (count > kListCap) {
+      const uint32_t kk = count < a.k ? count : a.k;
+      // candidates in [lo, hi) with class < below, over the whole block
+      auto count_if = [&](uint32_t lo, uint32_t hi, uint32_t below) -> uint32_t {
+        uint32_t n = 0u;
+        if (mine)
+          for (uint32_t p = tid; p < packs; p += NT) {
+            float x[N];
+            load_pack(in, p * N, a.K, -kInf, x);
+#pragma unroll
+            for (uint32_t i = 0; i < N; ++i) {
+              const uint32_t key = score_key(x[i]);
+              n += key >= lo && key < hi && p * N + i < below;
+            }
+          }
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) n += __shfl_xor(n, d);
+        __syncthreads();
+        if (lane == 0u) ctl[2 + wave] = n;
+        __syncthreads();
+        uint32_t sum = 0u;
+        for (uint32_t w = 0; w < kWaves; ++w) sum += ctl[2 + w];
+        return sum;
+      };
+      uint32_t t = bound;  // raised to the kk-th largest key: bits below the bound's differing ones are tried from the top
+      {
+        uint32_t v = 0u;
+        for (int bit = 31; bit >= (int)low_bits<T>(); --bit) {
+          const uint32_t cand = v | (1u << bit);
+          if (cand <= bound || count_if(cand, 0xFFFFFFFFu, 0xFFFFFFFFu) >= kk) v = cand;
+        }
+        if (v > t) t = v;
+      }
+      const uint32_t above = t + (1u << low_bits<T>());
+      const uint32_t gt = count_if(above, 0xFFFFFFFFu, 0xFFFFFFFFu);
+      uint32_t last = 0u;
+      for (int bit = 19; bit >= 0; --bit) {  // (at most 2^20 classes)
+        const uint32_t cand = last + (1u << bit);
+        if (gt + count_if(t, above, cand) < kk) last = cand;
+      }
+      __syncthreads();
+      if (tid == 0u) ctl[1] = 0u;
+      __syncthreads();
+      if (mine)
+        for (uint32_t p = tid; p < packs; p += NT) {
+          float x[N];
+          load_pack(in, p * N, a.K, -kInf, x);
+#pragma unroll
+          for (uint32_t i = 0; i < N; ++i) {
+            const uint32_t key = score_key(x[i]), c = p * N + i;
+            if (key >= above || (key >= t && c <= last)) list[atomicAdd(&ctl[1], 1u) & (kListCap - 1u)] = candidate(key, c);
+          }
+        }
+      __syncthreads();
+      count = ctl[1];
+    }
+    for (uint32_t i = tid; i < (count > a.k ? count : a.k); i += NT) {
+      if (i >= count) {
+        write_nothing(a, row, i);
+        continue;
+      }
+      const uint64_t v = list[i];
+      uint32_t rank = 0u;
+      for (uint32_t j = 0; j < count; ++j) rank += list[j] > v;
+      if (rank < a.k) write_candidate(a, row, rank, v);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------
+// distill.  With z = student / T, S = the listed classes, m_o, s_o = (largest score, sum of exp((x - m_o) / T)) over the classes OUTSIDE
+// S, and everything of a row's own (2 k exponentials) in 64 bits:
+//   Z = s_o e^((m_o - M) / T) + sum_S e^((x_c - M) / T),  p_R = its first summand / Z,  log p_c = (x_c - M) / T - log Z
+//   loss = sum_j q_j (log q_j - log p_(i_j)) + q_R (log q_R - log p_R)
+//   gradient outside S: p_c (Q - q_R / p_R) = e^((x_c - m_o) / T) * [(Q p_R - q_R) / s_o]     (one coefficient per row)
+//   gradient inside S:  p_c Q - sum of the class's q_j                                        (at most k per row)
+// The sums are kept apart because 1 - sum_S p and a loss near zero are differences of near numbers: p_R comes from its own sum, and an
+// error of s_o moves all p together so that it enters the loss times (p_R - q_R) only.
+// ---------------------------------------------------------------------------------------------------
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
+  return v;
+}
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) v = fmaxf(v, __shfl_xor(v, d));
+  return v;
+}
+
+// what the gradient's pass over the row needs: grad = coef * exp((x - m) / T) outside S
+struct RowGrad {
+  float m, coef;
+};
+
+constexpr int32_t kAgain = 1 << 30;  // on a class number: an earlier entry of the row lists the class already
+
+// a row's entries in LDS (k of each): e^((x - M) / T) of the student, the teacher's probability, the class (-1 = no entry), both scores
+struct Entries {
+  double *e, *q;
+  int32_t* id;
+  float *x, *t;
+  __device__ explicit Entries(uint32_t* base, uint32_t k) {
+    e = reinterpret_cast<double*>(base), q = e + k, id = reinterpret_cast<int32_t*>(q + k), x = reinterpret_cast<float*>(id + k), t = x + k;
+  }
+  static __host__ __device__ constexpr uint32_t words(uint32_t k) { return 7u * k; }
+};
+
+// one wave, one row: the teacher's entries against the student's row.  o = sums outside S.
+template <class T, bool GRAD>
+__device__ __forceinline__ RowGrad row_loss(const DistillArgs& a, uint64_t row, const Entries& en, uint32_t lane, const ExpSum& o) {
+  const double inv_T = 1.0 / a.temperature;
+  float xm = -FLT_MAX, tm = -FLT_MAX;
+  for (uint32_t j = lane; j < a.k; j += 64u)
+    if (en.id[j] >= 0) xm = fmaxf(xm, en.x[j]), tm = fmaxf(tm, en.t[j]);
+  const float M = wave_max(fmaxf(xm, o.m));
+  tm = wave_max(tm);
+  const double shift = a.lse ? (double)a.lse[row] : (double)tm * inv_T;
+  double zs = 0.0, ts = 0.0;
+  for (uint32_t j = lane; j < a.k; j += 64u)
+    if (en.id[j] >= 0) {
+      const double e = exp(((double)en.x[j] - (double)M) * inv_T), q = exp((double)en.t[j] * inv_T - shift);
+      en.e[j] = e, en.q[j] = q;
+      ts += q;
+      if (!(en.id[j] & kAgain)) zs += e;
+    }
+  zs = wave_sum(zs), ts = wave_sum(ts);
+  const double far = exp(((double)o.m - (double)M) * inv_T), Z = (double)o.s * far + zs, log_Z = log(Z);
+  // without lse the q are still to be divided by their sum
+  const double log_T = a.lse ? shift : shift + log(ts), scale = a.lse ? 1.0 : 1.0 / ts;
+  double Q = a.lse ? ts : 1.0, rest = 0.0, loss = 0.0;
+  for (uint32_t j = lane; j < a.k; j += 64u)
+    if (en.id[j] >= 0 && !(en.q[j] == 0.0))
+      loss += en.q[j] * scale * (((double)en.t[j] * inv_T - log_T) - (((double)en.x[j] - (double)M) * inv_T - log_Z));
+  loss = wave_sum(loss);
+  if (a.lse && o.s > 0.f && Q < 1.0) {
+    rest = 1.0 - Q;
+    loss += rest * (log(rest) - (((double)o.m - (double)M) * inv_T + log((double)o.s) - log_Z));
+    Q = 1.0;
+  }
+  if (a.loss && lane == 0u) a.loss[row] = (float)loss;
+  RowGrad g = {o.m, 0.f};
+  if (GRAD) {
+    const double w = (a.weight ? (double)a.weight[row * a.weight_stride] : 1.0) * inv_T;
+    // (nothing outside S: no gradient there; nothing in the whole row: NaN, as its softmax)
+    g.coef = !(o.s == 0.f) ? (float)((Q * far / Z - rest / (double)o.s) * w) : Z == 0.0 ? __builtin_nanf("") : 0.f;
+    T* out = static_cast<T*>(a.grad) + row * a.grad_stride;
+    for (uint32_t j = lane; j < a.k; j += 64u) {
+      const int32_t id = en.id[j];
+      if (id < 0 || (id & kAgain)) continue;
+      double qc = en.q[j];
+      for (uint32_t i = j + 1u; i < a.k; ++i)  // further entries of this class, in their order
+        if (en.id[i] == (id | kAgain)) qc += en.q[i];
+      out[id] = (T)(float)((en.e[j] / Z * Q - qc * scale) * w);
+    }
+  }
+  return g;
+}
+
+__host__ __device__ constexpr uint32_t distill_words(uint32_t K, uint32_t k, uint32_t threads) {  // LDS of a row, an even number
+  return (Entries::words(k) + 4u + 2u * (threads / 64u) + (K + 31u) / 32u + 1u) & ~1u;
+}
+
+// NT threads per row: 64 (a wave; 4 rows per block of 256) or the whole block.  The row is read once for the sums outside S -- S as a
+// bitmap in LDS, a pack's bits next to each other -- and, for the gradient, a second time, from whichever cache still holds it.
+template <class T, int NT, bool GRAD>
+__global__ __launch_bounds__(NT == 64 ? 256 : NT) void distill_kernel(const DistillArgs a) {
+  constexpr uint32_t N = Pack<T>::N, kGroups = NT == 64 ? 4 : 1, kWaves = NT / 64;
+  const uint32_t lane = threadIdx.x & 63u, group = NT == 64 ? threadIdx.x >> 6 : 0u, tid = NT == 64 ? lane : threadIdx.x;
+  const uint32_t words = (a.K + 31u) / 32u;
+  uint32_t* base = lds_words + group * distill_words(a.K, a.k, NT);
+  const Entries en(base, a.k);
+  uint32_t* ctl = base + Entries::words(a.k);            // [0] any entry, [1] any class twice, [2, 3] RowGrad
+  float* part = reinterpret_cast<float*>(ctl + 4);       // [2 * kWaves]
+  uint32_t* bitmap = ctl + 4 + 2u * kWaves;              // [words]
+  const uint32_t packs = (a.K + N - 1u) / N;
+  const float c2 = (float)(1.4426950408889634 / a.temperature);
+  auto sync = [] {
+    if (NT == 64) {
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    } else {
+      __syncthreads();
+    }
+  };
+  for (uint64_t row = (uint64_t)blockIdx.x * kGroups + group; row < a.n; row += (uint64_t)gridDim.x * kGroups) {
+    const T* in = static_cast<const T*>(a.in) + row * a.stride;
+    T* out = static_cast<T*>(a.grad) + row * a.grad_stride;
+    sync();  // the row before is done with the LDS
+    for (uint32_t i = tid; i < words; i += NT) bitmap[i] = 0u;
+    if (tid < 2u) ctl[tid] = 0u;
+    sync();
+    for (uint32_t j = tid; j < a.k; j += NT) {
+      int32_t id = a.ids[row * a.teacher_stride + j];
+      if ((uint32_t)id >= a.K) id = -1;
+      en.id[j] = id;
+      if (id >= 0) {
+        en.t[j] = a.values[row * a.teacher_stride + j], en.x[j] = (float)in[id];
+        ctl[0] = 1u;
+        if (atomicOr(&bitmap[id >> 5], 1u << (id & 31)) >> (id & 31) & 1u) ctl[1] = 1u;
+      }
+    }
+    sync();
+    if (ctl[0] == 0u) {  // no entry: nothing to learn from this row
+      if (tid == 0u && a.loss) a.loss[row] = 0.f;
+      if (GRAD) {
+        const float zero[N] = {};
+        for (uint32_t p = tid; p < packs; p += NT) store_pack(out, p * N, a.K, zero);
+      }
+      continue;
+    }
+    if (ctl[1]) {  // mark the entries whose class stands in front of them already
+      for (uint32_t j0 = 0; j0 < a.k; j0 += NT) {
+        const uint32_t j = j0 + tid;
+        bool again = false;
+        if (j < a.k && en.id[j] >= 0)
+          for (uint32_t i = 0; i < j; ++i) again |= (en.id[i] & ~kAgain) == en.id[j];
+        sync();
+        if (again) en.id[j] |= kAgain;
+        sync();
+      }
+    }
+    ExpSum o;
+    for (uint32_t p = tid; p < packs; p += NT) {
+      float x[N];
+      load_pack(in, p * N, a.K, -kInf, x);
+      const uint32_t bits = bitmap[p * N >> 5] >> (p * N & 31u);
+      if (bits & ((1u << N) - 1u)) {
+#pragma unroll
+        for (uint32_t i = 0; i < N; ++i) x[i] = (bits >> i) & 1u ? -kInf : x[i];
+      }
+      o.add(x, c2);
+    }
+    o.reduce_wave(c2);
+    if (NT > 64) {
+      if (lane == 0u) part[2 * (tid >> 6)] = o.m, part[2 * (tid >> 6) + 1] = o.s;
+      sync();
+    }
+    if (tid < 64u) {
+      if (NT > 64) {
+        o.m = lane < kWaves ? part[2 * lane] : -FLT_MAX, o.s = lane < kWaves ? part[2 * lane + 1] : 0.f;
+        o.reduce_wave(c2);
+      }
+      const RowGrad g = row_loss<T, GRAD>(a, row, en, lane, o);
+      if (GRAD && lane == 0u) ctl[2] = __float_as_uint(g.m), ctl[3] = __float_as_uint(g.coef);
+    }
+    if (GRAD) {
+      sync();
+      const float m = __uint_as_float(ctl[2]), coef = __uint_as_float(ctl[3]);
+      for (uint32_t p = tid; p < packs; p += NT) {
+        float x[N];
+        load_pack(in, p * N, a.K, -kInf, x);
+        const uint32_t bits = bitmap[p * N >> 5] >> (p * N & 31u);
+#pragma unroll
+        for (uint32_t i = 0; i < N; ++i) x[i] = coef * exp2_fast((x[i] - m) * c2);
+        if (bits & ((1u << N) - 1u)) {  // the listed classes of this pack are written already
+#pragma unroll
+          for (uint32_t i = 0; i < N; ++i)
+            if (p * N + i < a.K && !((bits >> i) & 1u)) out[p * N + i] = (T)x[i];
+        } else {
+          store_pack(out, p * N, a.K, x);
+        }
+      }
+    }
+  }
+}
+
+// up to 32 classes: a thread per row, rows staged in LDS and their gradients collected there in fp32
+template <class T, bool GRAD>
+__global__ __launch_bounds__(256) void distill_thread_kernel(const DistillArgs a) {
+  T* stage = reinterpret_cast<T*>(lds_words);
+  const uint32_t pitch = staged_pitch<T>(a.K), gpitch = a.K | 1u;
+  float* gstage = reinterpret_cast<float*>(lds_words + (256u * pitch * sizeof(T)) / 4u);
+  const double inv_T = 1.0 / a.temperature;
+  const float c2 = (float)(1.4426950408889634 / a.temperature);
+  for (uint64_t r0 = (uint64_t)blockIdx.x * 256u; r0 < a.n; r0 += (uint64_t)gridDim.x * 256u) {
+    const uint32_t rows = (uint32_t)(a.n - r0 < 256u ? a.n - r0 : 256u);
+    __syncthreads();
+    stage_rows(static_cast<const T*>(a.in), r0, rows, a.K, a.stride, stage, pitch);
+    __syncthreads();
+    if (threadIdx.x < rows) {
+      const uint64_t row = r0 + threadIdx.x;
+      const T* x = stage + threadIdx.x * pitch;
+      float* g = gstage + threadIdx.x * gpitch;
+      const int32_t* ids = a.ids + row * a.teacher_stride;
+      const float* tv = a.values + row * a.teacher_stride;
+      uint32_t listed = 0u, entries = 0u;
+      float tm = -FLT_MAX;
+      for (uint32_t j = 0; j < a.k; ++j)
+        if ((uint32_t)ids[j] < a.K) listed |= 1u << ids[j], tm = fmaxf(tm, tv[j]), ++entries;
+      if (listed == 0u) {
+        if (a.loss) a.loss[row] = 0.f;
+        if (GRAD)
+          for (uint32_t c = 0; c < a.K; ++c) g[c] = 0.f;
+      } else {
+        float om = -FLT_MAX, sm = -FLT_MAX;
+        for (uint32_t c = 0; c < a.K; ++c) {
+          const float v = (float)x[c];
+          if ((listed >> c) & 1u) sm = fmaxf(sm, v);
+          else om = fmaxf(om, v);
+        }
+        const float M = fmaxf(om, sm);
+        float os = 0.f;
+        double zs = 0.0;
+        for (uint32_t c = 0; c < a.K; ++c) {
+          const float v = (float)x[c];
+          if ((listed >> c) & 1u) zs += exp(((double)v - (double)M) * inv_T);
+          else os += exp2_fast((v - om) * c2);
+        }
+        const double far = exp(((double)om - (double)M) * inv_T), Z = (double)os * far + zs, log_Z = log(Z);
+        const double lse = a.lse ? (double)a.lse[row] : 0.0;
+        double ts = 0.0;
+        for (uint32_t j = 0; j < a.k; ++j)
+          if ((uint32_t)ids[j] < a.K) ts += a.lse ? exp((double)tv[j] * inv_T - lse) : exp(((double)tv[j] - (double)tm) * inv_T);
+        const double log_T = a.lse ? lse : (double)tm * inv_T + log(ts);
+        double Q = a.lse ? ts : 1.0, rest = 0.0, loss = 0.0;
+        if (a.lse && os > 0.f && Q < 1.0) {
+          rest = 1.0 - Q;
+          loss = rest * (log(rest) - (((double)om - (double)M) * inv_T + log((double)os) - log_Z));
+          Q = 1.0;
+        }
+        const double w = GRAD ? (a.weight ? (double)a.weight[row * a.weight_stride] : 1.0) * inv_T : 0.0;
+        if (GRAD) {
+          const float coef = !(os == 0.f) ? (float)((Q * far / Z - rest / (double)os) * w) : Z == 0.0 ? __builtin_nanf("") : 0.f;
+          for (uint32_t c = 0; c < a.K; ++c)
+            if (!((listed >> c) & 1u)) g[c] = coef * exp2_fast(((float)x[c] - om) * c2);
+        }
+        const bool repeats = entries != (uint32_t)__popc(listed);
+        uint32_t open = listed;  // classes of the list whose gradient is still to be written
+        for (uint32_t j = 0; j < a.k; ++j)
+          if ((uint32_t)ids[j] < a.K) {
+            const uint32_t c = (uint32_t)ids[j];
+            const double lq = (double)tv[j] * inv_T - log_T, q = exp(lq), z = ((double)(float)x[c] - (double)M) * inv_T;
+            if (!(q == 0.0)) loss += q * (lq - (z - log_Z));
+            if (GRAD && ((open >> c) & 1u)) {
+              open &= ~(1u << c);
+              double qc = q;
+              if (repeats)
+                for (uint32_t i = j + 1u; i < a.k; ++i)
+                  if (ids[i] == (int32_t)c) qc += exp((double)tv[i] * inv_T - log_T);
+              g[c] = (float)((exp(z) / Z * Q - qc) * w);
+            }
+          }
+        if (a.loss) a.loss[row] = (float)loss;
+      }
+    }
+    if (GRAD) {
+      __syncthreads();
+      T* out = static_cast<T*>(a.grad);
+      if (a.grad_stride == a.K && a.K > 1u) {
+        constexpr uint32_t N = Pack<T>::N;
+        const uint32_t total = rows * a.K, magic = (uint32_t)((0x100000000ull + a.K - 1u) / a.K);
+        T* dst = out + r0 * a.K;
+        for (uint32_t i = threadIdx.x * N; i < total; i += 256u * N) {
+          uint32_t r = __umulhi(i, magic), c = i - r * a.K;
+          float v[N];
+#pragma unroll
+          for (uint32_t j = 0; j < N; ++j) {
+            v[j] = i + j < total ? gstage[r * gpitch + c] : 0.f;
+            if (++c == a.K) c = 0u, ++r;
+          }
+          store_pack(dst, i, total, v);
+        }
+      } else {
+        for (uint32_t r = threadIdx.x >> 5; r < rows; r += 8u)
+          for (uint32_t c = threadIdx.x & 31u; c < a.K; c += 32u) out[(r0 + r) * a.grad_stride + c] = (T)gstage[r * gpitch + c];
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------
+// launches
+// ---------------------------------------------------------------------------------------------------
+template <class Kern, class... Args>
+hipError_t launch(Kern kern, uint64_t blocks, uint32_t threads, uint32_t lds, hipStream_t s, const Args&... args) {
+  (void)hipGetLastError();  // do not inherit a stale error
+  if (lds > 64u * 1024u) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (e != hipSuccess) return e;
+  }
+  constexpr uint64_t kMaxBlocks = 1u << 20;  // every kernel strides over the rest
+  hipLaunchKernelGGL(kern, dim3((uint32_t)(blocks < kMaxBlocks ? blocks : kMaxBlocks)), dim3(threads), lds, s, args...);
+  return hipGetLastError();
+}
+
+template <class T>
+hipError_t adjust_typed(const AdjustArgs& a, bool class_major, hipStream_t s) {
+  constexpr uint32_t N = Pack<T>::N;
+  AdjustTiles t{};
+  if (class_major) {
+    // without histories a tile is 256 packs of rows times all its classes; the counters of a history are 64 rows wide
+    t.rows = a.history ? 64u : 256u * N;
+    t.classes = a.K < (a.history ? 256u : 16u) ? a.K : (a.history ? 256u : 16u);
+    t.class_tiles = (a.K + t.classes - 1) / t.classes;
+    t.tiles = (a.n + t.rows - 1) / t.rows * t.class_tiles;
+    if (a.history) return launch(adjust_classes_kernel<T, true>, t.tiles, 256, t.rows * t.classes * 4u, s, a, t);
+    return launch(adjust_classes_kernel<T, false>, t.tiles, 256, 0, s, a, t);
+  }
+  const uint64_t row_packs = (a.K + N - 1) / N;
+  const uint32_t budget = a.n * row_packs < (1u << 20) ? 256u : 1024u;  // packs per tile
+  const uint32_t ppr = (uint32_t)(row_packs < budget ? row_packs : budget);
+  t.classes = ppr * N;
+  t.rows = budget / ppr;
+  t.magic = ppr > 1u ? (uint32_t)((0x100000000ull + ppr - 1u) / ppr) : 0u;
+  t.class_tiles = (row_packs + ppr - 1) / ppr;
+  t.tiles = (a.n + t.rows - 1) / t.rows * t.class_tiles;
+  if (a.history) return launch(adjust_rows_kernel<T, true>, t.tiles, 256, t.rows * t.classes * 4u, s, a, t);
+  return launch(adjust_rows_kernel<T, false>, t.tiles, 256, 0, s, a, t);
+}
+
+template <class T, bool CM>
+hipError_t top_thread(const TopArgs& a, hipStream_t s) {
+  const uint64_t blocks = (a.n + 255) / 256;
+  const uint32_t lds = CM ? 0u : 256u * (uint32_t)sizeof(T) * ((((a.K + 4 / sizeof(T) - 1) / (4 / sizeof(T))) | 1u) * (uint32_t)(4 / sizeof(T)));
+  if (a.k == 1u) return launch(top_thread_kernel<T, CM, 1>, blocks, 256, lds, s, a);
+  if (a.k == 2u) return launch(top_thread_kernel<T, CM, 2>, blocks, 256, lds, s, a);
+  if (a.k <= 4u) return launch(top_thread_kernel<T, CM, 4>, blocks, 256, lds, s, a);
+  return launch(top_thread_kernel<T, CM, 8>, blocks, 256, lds, s, a);
+}
+template <class T, bool CM>
+hipError_t top_wave(const TopArgs& a, hipStream_t s) {
+  constexpr uint32_t N = Pack<T>::N, rows = top_wave_rows(CM), threads = top_wave_waves(CM) * 64u;
+  const uint64_t blocks = (a.n + rows - 1) / rows;
+  const uint32_t lds = top_wave_waves(CM) * a.k * 8u + (CM ? a.K * 16u * (uint32_t)sizeof(T) : 0u), packs = (a.K + N - 1) / N;
+  if (packs <= 64u) return launch(top_wave_kernel<T, CM, 1>, blocks, threads, lds, s, a);
+  if (packs <= 128u) return launch(top_wave_kernel<T, CM, 2>, blocks, threads, lds, s, a);
+  if (packs <= 256u) return launch(top_wave_kernel<T, CM, 4>, blocks, threads, lds, s, a);
+  if constexpr (N == 4) return launch(top_wave_kernel<T, CM, 8>, blocks, threads, lds, s, a);
+  return hipErrorInvalidValue;
+}
+template <class T, int NT>
+hipError_t top_block(const TopArgs& a, hipStream_t s) {
+  return launch(top_block_kernel<T, NT>, a.n, NT, 8u * kListCap + 4u * NT + 8u * (NT / 64) + 4u * (2u + NT / 64), s, a);
+}
+template <class T>
+hipError_t top_typed(const TopArgs& a, bool class_major, hipStream_t s) {
+  if (a.K <= 32u && a.k <= 8u) return class_major ? top_thread<T, true>(a, s) : top_thread<T, false>(a, s);
+  if (class_major) return a.K <= kTopMaxClassMajor ? top_wave<T, true>(a, s) : hipErrorInvalidValue;
+  if (a.K <= 2048u) return top_wave<T, false>(a, s);
+  return a.K <= 16384u ? top_block<T, 256>(a, s) : top_block<T, 1024>(a, s);
+}
+
+template <class T, int NT, bool GRAD>
+hipError_t distill_rows(const DistillArgs& a, hipStream_t s) {
+  constexpr uint32_t groups = NT == 64 ? 4u : 1u;
+  const uint32_t lds = groups * 4u * distill_words(a.K, a.k, NT);
+  return launch(distill_kernel<T, NT, GRAD>, (a.n + groups - 1) / groups, NT == 64 ? 256 : NT, lds, s, a);
+}
+template <class T, bool GRAD>
+hipError_t distill_typed(const DistillArgs& a, hipStream_t s) {
+  constexpr uint32_t per_word = 4 / sizeof(T);
+  if (a.K <= 32u) {
+    const uint32_t pitch = (((a.K + per_word - 1) / per_word) | 1u) * per_word;
+    return launch(distill_thread_kernel<T, GRAD>, (a.n + 255) / 256, 256, 256u * (pitch * (uint32_t)sizeof(T) + (GRAD ? (a.K | 1u) * 4u : 0u)), s, a);
+  }
+  if (a.K <= 2048u) return distill_rows<T, 64, GRAD>(a, s);
+  return a.K <= 16384u ? distill_rows<T, 256, GRAD>(a, s) : distill_rows<T, 1024, GRAD>(a, s);
+}
+
+}  // namespace
+
+hipError_t launch_adjust(const AdjustArgs& a, uint32_t dtype, bool class_major, hipStream_t s) {
+  if (a.n == 0) return hipSuccess;
+  if (dtype == DDT_FP32) return adjust_typed<float>(a, class_major, s);
+  return dtype == DDT_FP16 ? adjust_typed<_Float16>(a, class_major, s) : adjust_typed<__bf16>(a, class_major, s);
+}
+hipError_t launch_top(const TopArgs& a, uint32_t dtype, bool class_major, hipStream_t s) {
+  if (a.n == 0) return hipSuccess;
+  if (dtype == DDT_FP32) return top_typed<float>(a, class_major, s);
+  return dtype == DDT_FP16 ? top_typed<_Float16>(a, class_major, s) : top_typed<__bf16>(a, class_major, s);
+}
+hipError_t launch_distill(const DistillArgs& a, uint32_t dtype, hipStream_t s) {
+  if (a.n == 0) return hipSuccess;
+  if (dtype == DDT_FP32) return a.grad ? distill_typed<float, true>(a, s) : distill_typed<float, false>(a, s);
+  if (dtype == DDT_FP16) return a.grad ? distill_typed<_Float16, true>(a, s) : distill_typed<_Float16, false>(a, s);
+  return a.grad ? distill_typed<__bf16, true>(a, s) : distill_typed<__bf16, false>(a, s);
+}
+
+}  // namespace ddt

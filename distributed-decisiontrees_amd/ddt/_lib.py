@@ -25,6 +25,7 @@ SYMBOLS = [
     "ddt_host_register", "ddt_host_unregister",
     "ddt_comm_create_hybrid", "ddt_comm_layout", "ddt_hybrid_rows", "ddt_score_hybrid_device", "ddt_classify_hybrid_device", "ddt_comm_abort",
     "ddt_group_create_hybrid",
+    "ddt_adjust_scores_device", "ddt_top_scores_device", "ddt_distill_device", "ddt_distill_grad_device",
 ]
 
 
@@ -56,6 +57,29 @@ class Info(C.Structure):
         ("num_cus", C.c_uint32), ("clock_khz", C.c_uint32), ("lds_bytes_per_cu", C.c_uint32), ("prepass_groups", C.c_uint32),
         ("fallback_kernel", C.c_uint32), ("build_checks", C.c_uint32),
     ]
+
+
+class Scores(C.Structure):
+    """ddt_scores_t (include/ddt.h): a matrix of class scores on the device"""
+
+    _fields_ = [("data", C.c_void_p), ("rows", C.c_uint64), ("row_stride", C.c_uint64), ("class_stride", C.c_uint64),
+                ("num_classes", C.c_uint32), ("dtype", C.c_uint32)]
+
+
+class Adjust(C.Structure):
+    """ddt_adjust_t"""
+
+    _fields_ = [("bias", C.c_void_p), ("bias_row_stride", C.c_uint64), ("bias_class_stride", C.c_uint64),
+                ("allowed", C.c_void_p), ("allowed_row_stride", C.c_uint64),
+                ("history", C.c_void_p), ("history_first", C.c_void_p), ("history_len", C.c_uint64), ("history_prompt", C.c_void_p),
+                ("repetition", C.c_void_p), ("frequency", C.c_void_p), ("presence", C.c_void_p)]
+
+
+class Teacher(C.Structure):
+    """ddt_teacher_t"""
+
+    _fields_ = [("ids", C.c_void_p), ("values", C.c_void_p), ("row_stride", C.c_uint64), ("lse", C.c_void_p), ("k", C.c_uint32),
+                ("temperature", C.c_double)]
 
 
 class Stats(C.Structure):
@@ -94,8 +118,19 @@ def lib():
         import torch  # noqa: F401
     except Exception:  # pragma: no cover - torch is optional for the pure C-ABI use
         pass
-    _lib = bind(C.CDLL(LIB_PATH))
+    _lib = bind_class_scores(bind(C.CDLL(LIB_PATH)))
     return _lib
+
+
+def bind_class_scores(L):
+    """Prototypes of the class-score operators (csrc/ddt_classes.cpp; a build of the host side may stand without them)."""
+    vp, PS = C.c_void_p, C.POINTER(Scores)
+    L.ddt_adjust_scores_device.restype, L.ddt_adjust_scores_device.argtypes = C.c_int, [vp, PS, C.POINTER(Adjust), PS, vp]
+    L.ddt_top_scores_device.restype, L.ddt_top_scores_device.argtypes = C.c_int, [vp, PS, C.c_uint32, C.c_double, vp, vp, vp, vp]
+    L.ddt_distill_device.restype, L.ddt_distill_device.argtypes = C.c_int, [vp, PS, C.POINTER(Teacher), vp, vp]
+    L.ddt_distill_grad_device.restype = C.c_int
+    L.ddt_distill_grad_device.argtypes = [vp, PS, C.POINTER(Teacher), vp, C.c_uint64, vp, PS, vp]
+    return L
 
 
 def bind(L):

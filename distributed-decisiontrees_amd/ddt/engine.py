@@ -103,6 +103,34 @@ def synth_tuples_host(row0: int, n: int, F: int, dist: int = 0, missing_bits: in
     return out
 
 
+_distill_cls = None
+
+
+def _distill_function():
+    """The torch.autograd.Function behind Engine.distill (made on first use: torch is imported where it is needed)."""
+    global _distill_cls
+    if _distill_cls is None:
+        import torch
+
+        class Distill(torch.autograd.Function):
+            @staticmethod
+            def forward(ctx, engine, student, ids, values, lse, temperature):
+                ctx.engine, ctx.temperature = engine, temperature
+                ctx.save_for_backward(student, ids, values, lse)
+                return engine.distill_device(student, ids, values, lse, temperature)
+
+            @staticmethod
+            @torch.autograd.function.once_differentiable
+            def backward(ctx, weight):
+                student, ids, values, lse = ctx.saved_tensors
+                # the loss comes out of the same pass once more (n floats); nothing but the inputs is kept between the passes
+                _, grad = ctx.engine.distill_grad_device(student, ids, values, lse, weight, ctx.temperature)
+                return None, grad, None, None, None, None
+
+        _distill_cls = Distill
+    return _distill_cls
+
+
 class Engine:
     """One engine == one GPU (the analogue of one FPGA running DTInference)."""
 
@@ -203,6 +231,191 @@ class Engine:
         s = torch.cuda.current_stream(class_scores.device) if stream is None else stream
         self._check(self._L.ddt_argmax_device(self._h, class_scores.data_ptr(), K, n, labels.data_ptr(), s.cuda_stream))
         return labels
+
+    # ---- class scores: after the trees ---------------------------------------------------------------
+    # Matrices are torch tensors [num_classes, n] as classify_device returns them; row-major logits [n, num_classes] go in as
+    # logits.t() (a view: the strides say which it is).  Everything is asynchronous on `stream` (default: the device's current
+    # one); results that are not handed in are allocated on it.
+    def _tensor(self, t, what: str, dtype=None, dim=None, shape=None):
+        import torch
+
+        if t.device.type != "cuda" or t.device.index != self.device:
+            raise ValueError(f"{what}: on {t.device}, the engine is on cuda:{self.device}")
+        if dtype is not None and t.dtype not in (dtype if isinstance(dtype, tuple) else (dtype,)):
+            raise ValueError(f"{what}: {t.dtype}, must be {dtype}")
+        if dim is not None and t.dim() != dim:
+            raise ValueError(f"{what}: {t.dim()} dimensions, must be {dim}")
+        if shape is not None and tuple(t.shape) != tuple(shape):
+            raise ValueError(f"{what}: shape {tuple(t.shape)}, must be {tuple(shape)}")
+        return t
+
+    def _packed(self, t, what: str, dtype, shape) -> int:
+        self._tensor(t, what, dtype, shape=shape)
+        if not t.is_contiguous():
+            raise ValueError(f"{what}: must be contiguous")
+        return t.data_ptr()
+
+    def _scores(self, t, what: str) -> _lib.Scores:
+        import torch
+
+        types = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+        self._tensor(t, what, tuple(types), 2)
+        K, n = t.shape
+        return _lib.Scores(t.data_ptr(), n, t.stride(1), t.stride(0), K, types[t.dtype])
+
+    def _on(self, stream):
+        """(context that allocates on the stream, its handle)"""
+        import contextlib
+
+        import torch
+
+        if stream is None:
+            return contextlib.nullcontext(), torch.cuda.current_stream(self.device).cuda_stream
+        return torch.cuda.stream(stream), stream.cuda_stream
+
+    def adjust_device(self, class_scores, bias=None, allowed=None, history=None, history_first=None, history_prompt=None,
+                      repetition=None, frequency=None, presence=None, out=None, stream=None):
+        """Penalties for repeated classes, biases and a mask on class scores [K, n] (fp32, fp16, bf16) -> adjusted scores, same type
+        and layout (ddt_adjust_scores_device; `out` may be `class_scores`).
+
+        bias            fp32 [K] (the base scores of an imported model, say) or [K, n], any strides
+        allowed         int32 / uint32 bits, class c at bit c % 32 of word c // 32: [ceil(K / 32)] or [n, ceil(K / 32)]; others get -inf
+        history         int32 classes; row r's are history[history_first[r] : history_first[r + 1]] (int64 [n + 1]), the first
+                        history_prompt[r] (int32 [n]) of them its prompt part
+        repetition      fp32 [n]: a class of the history: score / it if positive, else score * it
+        frequency       fp32 [n]: minus it for every time the class stands behind the prompt part
+        presence        fp32 [n]: minus it if it stands there at all"""
+        import torch
+
+        s = self._scores(class_scores, "class_scores")
+        K, n = class_scores.shape
+        a, f32, i32 = _lib.Adjust(), torch.float32, torch.int32
+        if bias is not None:
+            self._tensor(bias, "bias", f32)
+            if tuple(bias.shape) == (K,):
+                a.bias_class_stride = bias.stride(0)
+            elif tuple(bias.shape) == (K, n):
+                a.bias_class_stride, a.bias_row_stride = bias.stride()
+            else:
+                raise ValueError(f"bias: shape {tuple(bias.shape)}, must be {(K,)} or {(K, n)}")
+            a.bias = bias.data_ptr()
+        if allowed is not None:
+            words = (K + 31) // 32
+            self._tensor(allowed, "allowed", (i32, torch.uint32))
+            if tuple(allowed.shape) not in ((words,), (n, words)):
+                raise ValueError(f"allowed: shape {tuple(allowed.shape)}, must be {(words,)} or {(n, words)}")
+            if words > 1 and allowed.stride(-1) != 1:
+                raise ValueError("allowed: the words of a row must be contiguous")
+            a.allowed, a.allowed_row_stride = allowed.data_ptr(), allowed.stride(0) if allowed.dim() == 2 and n > 1 else 0
+        if history is not None:
+            if history_first is None:
+                raise ValueError("history without history_first")
+            a.history = self._packed(history, "history", i32, (history.numel(),))
+            a.history_len = history.numel()
+            a.history_first = self._packed(history_first, "history_first", torch.int64, (n + 1,))
+            if history_prompt is not None:
+                a.history_prompt = self._packed(history_prompt, "history_prompt", i32, (n,))
+            for name, t in (("repetition", repetition), ("frequency", frequency), ("presence", presence)):
+                if t is not None:
+                    setattr(a, name, self._packed(t, name, f32, (n,)))
+        elif any(t is not None for t in (history_first, history_prompt, repetition, frequency, presence)):
+            raise ValueError("history_first, history_prompt and penalties need a history")
+        on, handle = self._on(stream)
+        with on:
+            if out is None:
+                out = torch.empty_strided((K, n), (1, K) if s.class_stride == 1 and (s.row_stride >= K or n <= 1) else (n, 1),
+                                          dtype=class_scores.dtype, device=class_scores.device)
+            o = self._scores(out, "out")
+            self._check(self._L.ddt_adjust_scores_device(self._h, C.byref(s), C.byref(a), C.byref(o), handle))
+        return out
+
+    def top_device(self, class_scores, k: int, temperature: float = 1.0, ids=None, values=None, lse=None, stream=None):
+        """The k best classes of each row of class scores [K, n], best first, equal scores in the order of the classes ->
+        (ids int32 [n, k], values fp32 [n, k], lse fp32 [n] = log sum exp(score / temperature) over all classes): the class's
+        probability is exp(values / temperature - lse).  Rows with fewer candidates (NaN and -inf are none) end in id -1, value
+        -inf.  (ddt_top_scores_device)"""
+        import torch
+
+        s = self._scores(class_scores, "class_scores")
+        n, dev = class_scores.shape[1], class_scores.device
+        on, handle = self._on(stream)
+        with on:
+            ids = torch.empty((n, k), dtype=torch.int32, device=dev) if ids is None else ids
+            values = torch.empty((n, k), dtype=torch.float32, device=dev) if values is None else values
+            lse = torch.empty(n, dtype=torch.float32, device=dev) if lse is None else lse
+            self._check(self._L.ddt_top_scores_device(
+                self._h, C.byref(s), k, temperature, self._packed(ids, "ids", torch.int32, (n, k)),
+                self._packed(values, "values", torch.float32, (n, k)), self._packed(lse, "lse", torch.float32, (n,)), handle))
+        return ids, values, lse
+
+    def top_classes_device(self, d_tuples, k: int, temperature: float = 1.0, stream=None, **adjust):
+        """Tuple lines -> (ids, values, lse) of top_device: classify_device's class sums, adjust_device with the keywords given here
+        (bias = an imported model's base scores, allowed, histories ...), top_device.  k = 1 is the label; a larger k is what a
+        student network learns from (distill)."""
+        import contextlib
+
+        import torch
+
+        with contextlib.nullcontext() if stream is None else torch.cuda.stream(stream):
+            _, scores = self.classify_device(d_tuples, want_labels=False)
+            if adjust:
+                self.adjust_device(scores, out=scores, **adjust)
+            return self.top_device(scores, k, temperature)
+
+    def _teacher(self, student, ids, values, lse, temperature) -> _lib.Teacher:
+        import torch
+
+        n, k = student.shape[0], ids.shape[-1]
+        self._tensor(ids, "ids", torch.int32, shape=(n, k))
+        self._tensor(values, "values", torch.float32, shape=(n, k))
+        if (k > 1 and (ids.stride(1) != 1 or values.stride(1) != 1)) or (n > 1 and ids.stride(0) != values.stride(0)):
+            raise ValueError("ids, values: rows must be contiguous and stand equally far apart")
+        t = _lib.Teacher(ids.data_ptr(), values.data_ptr(), ids.stride(0) if n > 1 else k, None, k, temperature)
+        if lse is not None:
+            t.lse = self._packed(lse, "lse", torch.float32, (n,))
+        return t
+
+    def distill_device(self, student, ids, values, lse=None, temperature: float = 1.0, loss=None, stream=None):
+        """KL divergence of a student's softmax (scores [n, K], row-major) from a teacher's top scores (ids, values, lse of
+        top_device at the same temperature) -> loss fp32 [n].  lse None: the teacher's probabilities are normalised over the
+        listed classes; otherwise everything it does not list is one more outcome.  (ddt_distill_device)"""
+        import torch
+
+        s = self._scores(student.t() if student.dim() == 2 else student, "student")
+        t = self._teacher(student, ids, values, lse, temperature)
+        on, handle = self._on(stream)
+        with on:
+            loss = torch.empty(student.shape[0], dtype=torch.float32, device=student.device) if loss is None else loss
+            self._check(self._L.ddt_distill_device(self._h, C.byref(s), C.byref(t),
+                                                   self._packed(loss, "loss", torch.float32, (student.shape[0],)), handle))
+        return loss
+
+    def distill_grad_device(self, student, ids, values, lse=None, row_weight=None, temperature: float = 1.0, loss=None, grad=None,
+                            stream=None):
+        """distill_device and, from the same pass over the student's scores, the gradient of sum(row_weight * loss) by them ->
+        (loss fp32 [n], grad [n, K] of the student's type); row_weight fp32 [n] (any stride; None = 1), `grad` may be `student`.
+        (ddt_distill_grad_device)"""
+        import torch
+
+        s = self._scores(student.t() if student.dim() == 2 else student, "student")
+        t = self._teacher(student, ids, values, lse, temperature)
+        n = student.shape[0]
+        if row_weight is not None:
+            self._tensor(row_weight, "row_weight", torch.float32, shape=(n,))
+        on, handle = self._on(stream)
+        with on:
+            loss = torch.empty(n, dtype=torch.float32, device=student.device) if loss is None else loss
+            grad = torch.empty(student.shape, dtype=student.dtype, device=student.device) if grad is None else grad
+            g = self._scores(grad.t(), "grad")
+            self._check(self._L.ddt_distill_grad_device(
+                self._h, C.byref(s), C.byref(t), row_weight.data_ptr() if row_weight is not None else None,
+                row_weight.stride(0) if row_weight is not None and n > 1 else 0,
+                self._packed(loss, "loss", torch.float32, (n,)), C.byref(g), handle))
+        return loss, grad
+
+    def distill(self, student, ids, values, lse=None, temperature: float = 1.0):
+        """distill_device for training: loss fp32 [n] that autograd takes back to `student` (the teacher gets no gradient)."""
+        return _distill_function().apply(self, student, ids, values, lse, temperature)
 
     def set_option(self, key: str, value: int):
         self._check(self._L.ddt_set_option(self._h, key.encode(), int(value)))

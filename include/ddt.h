@@ -27,7 +27,7 @@
 extern "C" {
 #endif
 
-#define DDT_ABI_VERSION 6 /* 6: ddt_info::build_checks (was reserved), "sparse_r_*" kernels + option sparse_r32, ddt_debug_rank32_tables; 5: ddt_info grew (fallback_kernel); 4: hybrid jobs (ddt_comm_create_hybrid, ddt_score_hybrid_device, ...), ddt_comm_abort; 3: ddt_stats grew */
+#define DDT_ABI_VERSION 7 /* 7: class-score operators (ddt_adjust_scores_device, ddt_top_scores_device, ddt_distill*_device); 6: ddt_info::build_checks (was reserved), "sparse_r_*" kernels + option sparse_r32, ddt_debug_rank32_tables; 5: ddt_info grew (fallback_kernel); 4: hybrid jobs (ddt_comm_create_hybrid, ddt_score_hybrid_device, ...), ddt_comm_abort; 3: ddt_stats grew */
 
 /* Threading: an engine is not thread-safe -- calls on ONE engine must not overlap; different engines (also on the
  * same device) are independent.  ddt_*_device calls are asynchronous on the given stream; ddt_destroy and
@@ -188,6 +188,75 @@ int ddt_classify_device(ddt_engine* e, const void* d_tuple_lines, size_t n_tuple
 int ddt_classify(ddt_engine* e, const void* tuple_lines, size_t n_tuples, int32_t* labels, float* class_scores);
 int ddt_argmax_device(ddt_engine* e, const float* d_class_scores, uint32_t num_classes, size_t n, int32_t* d_labels,
                       void* hip_stream);
+
+/* -- class scores: what becomes of them after the trees (EXTENSIONS: the reference ends with the sum) -------------------
+ *    A matrix of scores on the device, row r (tuple), class c at data[r * row_stride + c * class_stride] (elements).  One of the strides is
+ *    1: class-major is what ddt_classify_device writes ([num_classes][n]: row_stride 1, class_stride n), row-major ([n][num_classes]:
+ *    class_stride 1) is how a network holds its logits.  Strides may leave gaps, rows / classes must not overlap, data must be aligned to
+ *    its element.  The calls need an engine (its device, its error text) but no loaded model, keep nothing, allocate nothing and only enqueue
+ *    on `hip_stream`: they may be captured.  Whatever the type, sums and exponentials are fp32 or wider and a result is rounded once.     -- */
+enum { DDT_FP32 = 0, DDT_FP16 = 1, DDT_BF16 = 2 };
+#define DDT_MAX_CLASSES (1u << 20)  /* classes these calls take */
+#define DDT_MAX_TOP 256             /* classes a teacher lists per row, and ddt_top_scores_device returns */
+typedef struct ddt_scores_t {
+  void*    data;
+  uint64_t rows, row_stride, class_stride;
+  uint32_t num_classes;
+  uint32_t dtype; /* DDT_FP32 / DDT_FP16 / DDT_BF16 */
+} ddt_scores_t;
+
+/* Adjusted scores.  With N = how often class c stands in row r's history and N' = how often behind the history's prompt part, in this order:
+ *      N  > 0:  x = x > 0 ? x / repetition[r] : x * repetition[r]
+ *               x = x - frequency[r] * N'
+ *      N' > 0:  x = x - presence[r]
+ *               x = x + bias(r, c)
+ *      class not allowed: -inf, whatever the score was (NaN included)
+ * Every array may be NULL (no bias; every class allowed; penalties 1, 0, 0; no prompt part).  A row that allows nothing becomes -inf. */
+typedef struct ddt_adjust_t {
+  const float*    bias;               /* bias(r, c) = bias[r * bias_row_stride + c * bias_class_stride]; stride 0 = the same for all, e.g. the
+                                         base scores of an imported model, [num_classes] with strides 0, 1                               */
+  uint64_t        bias_row_stride, bias_class_stride;
+  const uint32_t* allowed;            /* class c is allowed in row r: bit c % 32 of allowed[r * allowed_row_stride + c / 32]               */
+  uint64_t        allowed_row_stride; /* words; 0 = one mask for every row, else >= ceil(num_classes / 32)                                */
+  const int32_t*  history;            /* classes, history_len of them; a number outside 0 .. num_classes - 1 stands for no class           */
+  const int64_t*  history_first;      /* [rows + 1]: row r's history is [history_first[r], history_first[r + 1]), clamped to the array      */
+  uint64_t        history_len;
+  const int32_t*  history_prompt;     /* [rows]: that many entries at the front of the row's history are its prompt part                   */
+  const float    *repetition, *frequency, *presence; /* [rows]; without a history they do nothing                                           */
+} ddt_adjust_t;
+/* out has the shape, type and layout of in; out->data == in->data with the same strides works in place, other overlap is refused. */
+int ddt_adjust_scores_device(ddt_engine* e, const ddt_scores_t* in, const ddt_adjust_t* adjust, const ddt_scores_t* out, void* hip_stream);
+
+/* The k best classes of each row, best first, equal scores in the order of the classes: d_ids, d_values [rows][k].  NaN and -inf are never
+ * among them; a row with fewer candidates is filled up with id -1, value -inf.  d_lse [rows] (may be NULL): log sum_c exp(score / temperature)
+ * over ALL classes -- exp(value / temperature - lse) is the class's probability; -inf for a row of -inf, NaN for a row that holds a NaN (and
+ * no +inf).  k = 1 .. DDT_MAX_TOP, temperature 0.001 .. 1000.  Class-major matrices: up to 2048 classes (DDT_EUNSUPPORTED beyond).          */
+int ddt_top_scores_device(ddt_engine* e, const ddt_scores_t* scores, uint32_t k, double temperature, int32_t* d_ids, float* d_values,
+                          float* d_lse, void* hip_stream);
+
+/* A teacher's top scores, as ddt_top_scores_device leaves them: entry j of row r lists class ids[r * row_stride + j] with score
+ * values[r * row_stride + j]; an id outside 0 .. num_classes - 1 is no entry (a shorter list, a padded row).
+ *   q_j = exp(values / T - lse): its probability, with the rest q_R = 1 - sum q_j standing for all other classes together;
+ *   lse == NULL: q = softmax(values / T) over the row's entries, no rest.                                                                  */
+typedef struct ddt_teacher_t {
+  const int32_t* ids;
+  const float*   values;
+  uint64_t       row_stride; /* >= k */
+  const float*   lse;        /* [rows] or NULL; log sum exp(score / T) over all the teacher's classes, at the SAME temperature             */
+  uint32_t       k;          /* 1 .. DDT_MAX_TOP */
+  double         temperature; /* T of both, 0.001 .. 1000 */
+} ddt_teacher_t;
+/* Distillation loss of a student's scores (row-major), p = softmax(student / T):
+ *      loss[r] = sum_j q_j (log q_j - log p_(id j)) + q_R (log q_R - log p_R),   p_R = the student's probability of the classes not listed
+ * The rest is left out where q_R or p_R is 0.  A row without entries: 0.  A class listed twice counts with both entries.  A row of the
+ * student that holds NaN or +inf, or nothing but -inf, has no softmax: its loss and gradient are NaN.
+ * ..._grad: also grad (row-major, the student's type; may be the student's own buffer) =
+ *      row_weight[r] d loss[r] / d student[r][c] = row_weight[r] / T (p_c Q - sum of q_j with id c - [c not listed] q_R p_c / p_R),
+ *      Q = sum q_j + q_R; row_weight[r * row_weight_stride] (stride 0 = one for all; NULL = 1) is the gradient that arrives at loss[r].
+ *      d_loss may be NULL then.                                                                                                            */
+int ddt_distill_device(ddt_engine* e, const ddt_scores_t* student, const ddt_teacher_t* teacher, float* d_loss, void* hip_stream);
+int ddt_distill_grad_device(ddt_engine* e, const ddt_scores_t* student, const ddt_teacher_t* teacher, const float* row_weight,
+                            uint64_t row_weight_stride, float* d_loss, const ddt_scores_t* grad, void* hip_stream);
 
 /* -- sparse (explicit-children) model stream (deep random forests; an EXTENSION -- the reference
  *    only takes perfect trees of <= 16 levels whose 2^(D+1)-1 words fit a PU's BRAM, DTPU.sv:20-28; its own hook for
