@@ -18,6 +18,7 @@ namespace {
 extern __shared__ uint32_t lds_words[];
 
 constexpr float kInf = __builtin_inff();
+constexpr double kLog2e = 1.4426950408889634;
 
 template <class T>
 struct Pack {
@@ -57,6 +58,72 @@ __device__ __forceinline__ void store_pack(T* row, uint32_t c, uint32_t end, con
 // x ^ 2: the hardware instruction (1 ulp; results below 2^-126 may come back as 0 -- nothing next to a sum whose largest term is 1)
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// 2^y and ln v in 64 bits for the rows' own numbers.  2^y: y = n + f with |f| <= 1/2, the power series of e^(f ln 2) to the 11th power
+// (the 12th is below 7e-15 of the sum), scaled by 2^n: a third of the instructions of the library's exp, which aims at the last bit.
+__device__ __forceinline__ double exp2_64(double y) {
+  y = y < -1100.0 ? -1100.0 : y > 1100.0 ? 1100.0 : y;  // (NaN stays)
+  const double n = __builtin_rint(y), f = (y - n) * 0.69314718055994530942;
+  double p = 1.0 / 39916800.0;
+  p = fma(p, f, 1.0 / 3628800.0);
+  p = fma(p, f, 1.0 / 362880.0);
+  p = fma(p, f, 1.0 / 40320.0);
+  p = fma(p, f, 1.0 / 5040.0);
+  p = fma(p, f, 1.0 / 720.0);
+  p = fma(p, f, 1.0 / 120.0);
+  p = fma(p, f, 1.0 / 24.0);
+  p = fma(p, f, 1.0 / 6.0);
+  p = fma(p, f, 0.5);
+  p = fma(p, f, 1.0);
+  p = fma(p, f, 1.0);
+  return __builtin_amdgcn_ldexp(p, (int)n);
+}
+// ln v: the fp32 logarithm and one Newton step on 2^y = v.  For 0 and the normal fp32 range, which sums relative to their largest term
+// and probabilities that count stay in.
+__device__ __forceinline__ double log_64(double v) {
+  if (v == 0.0) return -__builtin_inf();
+  const double y = (double)__builtin_amdgcn_logf((float)v), r = fma(v, exp2_64(-y), -1.0);
+  return fma(y, 0.69314718055994530942, r - 0.5 * r * r);
+}
+
+// reductions over a wave: five moves within rows of 16 lanes and across them (DPP: no LDS), the last lane then holds the result of all
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp(float idle, float v) {
+  return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp((int)__float_as_uint(idle), (int)__float_as_uint(v), CTRL, ROWS, 0xF, false));
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp(double idle, double v) {
+  const uint64_t i = (uint64_t)__double_as_longlong(idle), b = (uint64_t)__double_as_longlong(v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp((int)(uint32_t)i, (int)(uint32_t)b, CTRL, ROWS, 0xF, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp((int)(uint32_t)(i >> 32), (int)(uint32_t)(b >> 32), CTRL, ROWS, 0xF, false);
+  return __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
+}
+constexpr int kRowShr1 = 0x111, kRowShr2 = 0x112, kRowShr4 = 0x114, kRowShr8 = 0x118, kRowBcast15 = 0x142, kRowBcast31 = 0x143;
+__device__ __forceinline__ float last_lane(float v) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), 63)); }
+__device__ __forceinline__ double last_lane(double v) {
+  const uint64_t b = (uint64_t)__double_as_longlong(v);
+  const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)b, 63), hi = __builtin_amdgcn_readlane((uint32_t)(b >> 32), 63);
+  return __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
+}
+template <class F>
+__device__ __forceinline__ F wave_sum(F v) {
+  v += dpp<kRowShr1, 0xF>((F)0, v);
+  v += dpp<kRowShr2, 0xF>((F)0, v);
+  v += dpp<kRowShr4, 0xF>((F)0, v);
+  v += dpp<kRowShr8, 0xF>((F)0, v);
+  v += dpp<kRowBcast15, 0xA>((F)0, v);
+  v += dpp<kRowBcast31, 0xC>((F)0, v);
+  return last_lane(v);
+}
+__device__ __forceinline__ float wave_max(float v) {
+  v = fmaxf(v, dpp<kRowShr1, 0xF>(v, v));
+  v = fmaxf(v, dpp<kRowShr2, 0xF>(v, v));
+  v = fmaxf(v, dpp<kRowShr4, 0xF>(v, v));
+  v = fmaxf(v, dpp<kRowShr8, 0xF>(v, v));
+  v = fmaxf(v, dpp<kRowBcast15, 0xA>(v, v));
+  v = fmaxf(v, dpp<kRowBcast31, 0xC>(v, v));
+  return last_lane(v);
+}
+
 // ---------------------------------------------------------------------------------------------------
 // adjust
 // ---------------------------------------------------------------------------------------------------
@@ -93,13 +160,33 @@ __device__ __forceinline__ void count_history(const AdjustArgs& a, uint64_t r0, 
     int64_t split = a.prompt ? (int64_t)a.prompt[r0 + r] : 0;
     split = split < 0 ? lo : split > hi - lo ? hi : lo + split;
     uint32_t* row = counts + r * row_pitch;
-    for (int64_t i = lo + lane; i < hi; i += step) {
-      const uint32_t c = (uint32_t)a.history[i] - c0;
-      if (c < C) {
-        if (i >= split) atomicAdd(&row[c * class_pitch], 1u);
-        else atomicOr(&row[c * class_pitch], kInPrompt);
+    // kAhead 16-byte loads of a thread in flight: every tile of the row reads the whole history (from L2), and one entry at a time
+    // that is 400 dependent loads for 100,000 entries
+    constexpr int kAhead = 4;
+    auto count_part = [&](int64_t from, int64_t to, bool in_prompt) {
+      for (int64_t i = from + 4 * lane; i < to; i += (int64_t)step * 4 * kAhead) {
+        uint32_t c[kAhead][4];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          const int64_t at = i + (int64_t)u * step * 4;
+          if (at + 4 <= to) __builtin_memcpy(c[u], a.history + at, 16);
+          else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) c[u][j] = at + j < to ? (uint32_t)a.history[at + j] : 0xFFFFFFFFu;
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (c[u][j] - c0 < C) {
+              if (in_prompt) atomicOr(&row[(c[u][j] - c0) * class_pitch], kInPrompt);
+              else atomicAdd(&row[(c[u][j] - c0) * class_pitch], 1u);
+            }
       }
-    }
+    };
+    count_part(lo, split, true);
+    count_part(split, hi, false);
   }
 }
 
@@ -248,19 +335,15 @@ struct ExpSum {
     for (uint32_t i = 0; i < N; ++i) t += exp2_fast((x[i] - m) * c);
     s += t;
   }
-  __device__ __forceinline__ void merge(float om, float os, float c) {
-    const float M = fmaxf(m, om);
-    s = s * exp2_fast((m - M) * c) + os * exp2_fast((om - M) * c);
+  __device__ __forceinline__ void reduce_wave(float c) {  // the same in every lane afterwards
+    const float M = wave_max(m);
+    s = wave_sum(s * exp2_fast((m - M) * c));
     m = M;
-  }
-  __device__ __forceinline__ void reduce_wave(float c) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) merge(__shfl_xor(m, d), __shfl_xor(s, d), c);
   }
 };
 __device__ __forceinline__ float log_sum(const ExpSum& e, double inv_T) {
   if (e.m == kInf) return kInf;
-  return (float)((double)e.m * inv_T + log((double)e.s));  // nothing but -inf: log 0 = -inf
+  return (float)((double)e.m * inv_T + log_64((double)e.s));  // nothing but -inf: log 0 = -inf
 }
 
 // ---------------------------------------------------------------------------------------------------
@@ -325,7 +408,7 @@ template <class T, bool CM, int KK>
 __global__ __launch_bounds__(256) void top_thread_kernel(const TopArgs a) {
   T* stage = reinterpret_cast<T*>(lds_words);
   const uint32_t pitch = staged_pitch<T>(a.K);
-  const float c2 = (float)(1.4426950408889634 / a.temperature);
+  const float c2 = (float)(kLog2e / a.temperature);
   const uint64_t step = (uint64_t)gridDim.x * 256u;
   for (uint64_t r0 = (uint64_t)blockIdx.x * 256u; r0 < a.n; r0 += step) {
     const uint32_t rows = (uint32_t)(a.n - r0 < 256u ? a.n - r0 : 256u);
@@ -385,6 +468,11 @@ __device__ __forceinline__ uint32_t wave_kth_key(const uint32_t (&key)[E], uint3
 
 // up to 2048 classes: a wave per row, all its keys in registers (P packs per lane).  Class-major rows are staged through LDS, 16 at a
 // time (64-byte pieces of fp32), for the 8 waves of the block.
+constexpr uint32_t kWaveList = 128;  // candidates that are ranked without an exact count
+__device__ __forceinline__ uint32_t lanes_below(uint64_t ballot) {
+  return __builtin_amdgcn_mbcnt_hi((uint32_t)(ballot >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)ballot, 0u));
+}
+__host__ __device__ constexpr uint32_t wave_list(uint32_t k) { return k > kWaveList ? k : kWaveList; }
 constexpr uint32_t top_wave_rows(bool class_major) { return class_major ? 16u : 4u; }
 constexpr uint32_t top_wave_waves(bool class_major) { return class_major ? 8u : 4u; }
 template <class T, bool CM, int P>
@@ -392,9 +480,9 @@ __global__ __launch_bounds__(top_wave_waves(CM) * 64) void top_wave_kernel(const
   constexpr int N = (int)Pack<T>::N, E = P * N;
   constexpr uint32_t kRows = top_wave_rows(CM), kWaves = top_wave_waves(CM);
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-  uint64_t* list = reinterpret_cast<uint64_t*>(lds_words) + wave * a.k;  // the wave's selected candidates
-  T* stage = reinterpret_cast<T*>(reinterpret_cast<uint64_t*>(lds_words) + kWaves * a.k);  // class-major: [K][16] scores
-  const float c2 = (float)(1.4426950408889634 / a.temperature);
+  uint64_t* list = reinterpret_cast<uint64_t*>(lds_words) + wave * wave_list(a.k);  // the wave's selected candidates
+  T* stage = reinterpret_cast<T*>(reinterpret_cast<uint64_t*>(lds_words) + kWaves * wave_list(a.k));  // class-major: [K][16] scores
+  const float c2 = (float)(kLog2e / a.temperature);
   for (uint64_t r0 = (uint64_t)blockIdx.x * kRows; r0 < a.n; r0 += (uint64_t)gridDim.x * kRows) {
     if (CM) {
       __syncthreads();
@@ -405,69 +493,97 @@ __global__ __launch_bounds__(top_wave_waves(CM) * 64) void top_wave_kernel(const
     }
     for (uint32_t rr = wave; rr < kRows && r0 + rr < a.n; rr += kWaves) {
       const uint64_t row = r0 + rr;
-      uint32_t key[E];
-      ExpSum e;
+      float x[E];
+      float best = -kInf;
 #pragma unroll
       for (int p = 0; p < P; ++p) {
         const uint32_t c = ((uint32_t)p * 64u + lane) * N;
-        float x[N];
+        float v[N];
         if (CM) {
 #pragma unroll
-          for (int i = 0; i < N; ++i) x[i] = c + i < a.K ? (float)stage[(c + i) * 16u + rr] : -kInf;
+          for (int i = 0; i < N; ++i) v[i] = c + i < a.K ? (float)stage[(c + i) * 16u + rr] : -kInf;
         } else {
-          load_pack(static_cast<const T*>(a.in) + row * a.stride, c, a.K, -kInf, x);
+          load_pack(static_cast<const T*>(a.in) + row * a.stride, c, a.K, -kInf, v);
         }
-        e.add(x, c2);
 #pragma unroll
-        for (int i = 0; i < N; ++i) key[p * N + i] = score_key(x[i]);
+        for (int i = 0; i < N; ++i) x[p * N + i] = v[i], best = fmaxf(best, v[i]);
       }
-      e.reduce_wave(c2);
+      ExpSum e;
+      e.m = fmaxf(wave_max(best), -FLT_MAX);
+#pragma unroll
+      for (int i = 0; i < E; ++i) e.s += exp2_fast((x[i] - e.m) * c2);
+      e.s = wave_sum(e.s);
       if (a.lse && lane == 0u) a.lse[row] = log_sum(e, 1.0 / a.temperature);
-      uint32_t valid = 0u;
+      // A bound that at least k scores reach: the k-th largest of the lanes' best, to 16 bits (sign, exponent, 7 bits: no more than a
+      // few scores stand between the exact one and this).  What reaches it is listed and ranked.
+      uint32_t count = kWaveList + 1u;
+      if (a.k <= 64u) {
+        const uint32_t lane_key[1] = {score_key(best)};
+        const uint32_t t = wave_kth_key(lane_key, a.k, 16u);
+        const float bound = t ? key_score(t) : -FLT_MAX;
+        count = 0u;
 #pragma unroll
-      for (int i = 0; i < E; ++i) valid += __popcll(__ballot(key[i] != 0u));
-      const uint32_t kk = valid < a.k ? valid : a.k;
-      uint32_t t = wave_kth_key(key, kk, low_bits<T>());
-      if (t == 0u) t = 1u;  // (fewer than k candidates: all of them)
-      // everything from t up, if that is kk; else what lies above t's score, and of the classes with t's score the lowest ones
-      uint32_t ge = 0u, gt = 0u;
-      const uint32_t above = t + (1u << low_bits<T>());
-#pragma unroll
-      for (int i = 0; i < E; ++i) ge += __popcll(__ballot(key[i] >= t)), gt += __popcll(__ballot(key[i] >= above));
-      uint32_t last = 0xFFFFFFFFu;  // highest class admitted among the equal ones
-      if (ge > kk) {
-        last = 0u;
-        for (int bit = 10; bit >= 0; --bit) {  // (at most 2048 classes)
-          const uint32_t cand = last + (1u << bit);
-          uint32_t cnt = gt;
+        for (int i = 0; i < E; ++i) count += __popcll(__ballot(x[i] >= bound));
+        if (count <= kWaveList) {
+          uint32_t base = 0u;
 #pragma unroll
           for (int i = 0; i < E; ++i) {
-            const uint32_t c = ((uint32_t)(i / N) * 64u + lane) * N + i % N;
-            cnt += __popcll(__ballot(key[i] >= t && key[i] < above && c < cand));
+            const bool take = x[i] >= bound;
+            const uint64_t b = __ballot(take);
+            if (b == 0u) continue;
+            if (take) list[base + lanes_below(b)] = candidate(score_key(x[i]), ((uint32_t)(i / N) * 64u + lane) * N + i % N);
+            base += __popcll(b);
           }
-          if (cnt < kk) last = cand;
         }
       }
-      uint32_t base = 0u;
+      if (count > kWaveList) {  // many wanted, or many that tie: count exactly, bit by bit
+        uint32_t key[E];
+        uint32_t valid = 0u;
 #pragma unroll
-      for (int i = 0; i < E; ++i) {
-        const uint32_t c = ((uint32_t)(i / N) * 64u + lane) * N + i % N;
-        const bool take = key[i] >= t && (key[i] >= above || c <= last);
-        const uint64_t b = __ballot(take);
-        if (take) list[base + __popcll(b & ((1ull << lane) - 1ull))] = candidate(key[i], c);
-        base += __popcll(b);
+        for (int i = 0; i < E; ++i) key[i] = score_key(x[i]), valid += __popcll(__ballot(key[i] != 0u));
+        const uint32_t kk = valid < a.k ? valid : a.k;
+        uint32_t t = wave_kth_key(key, kk, low_bits<T>());
+        if (t == 0u) t = 1u;  // (fewer than k candidates: all of them)
+        // everything from t up, if that is kk; else what lies above t's score, and of the classes with t's score the lowest ones
+        uint32_t ge = 0u, gt = 0u;
+        const uint32_t above = t + (1u << low_bits<T>());
+#pragma unroll
+        for (int i = 0; i < E; ++i) ge += __popcll(__ballot(key[i] >= t)), gt += __popcll(__ballot(key[i] >= above));
+        uint32_t last = 0xFFFFFFFFu;  // highest class admitted among the equal ones
+        if (ge > kk) {
+          last = 0u;
+          for (int bit = 10; bit >= 0; --bit) {  // (at most 2048 classes)
+            const uint32_t cand = last + (1u << bit);
+            uint32_t cnt = gt;
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+              const uint32_t c = ((uint32_t)(i / N) * 64u + lane) * N + i % N;
+              cnt += __popcll(__ballot(key[i] >= t && key[i] < above && c < cand));
+            }
+            if (cnt < kk) last = cand;
+          }
+        }
+        count = 0u;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          const uint32_t c = ((uint32_t)(i / N) * 64u + lane) * N + i % N;
+          const bool take = key[i] >= t && (key[i] >= above || c <= last);
+          const uint64_t b = __ballot(take);
+          if (take) list[count + lanes_below(b)] = candidate(key[i], c);
+          count += __popcll(b);
+        }
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
-      for (uint32_t i = lane; i < a.k; i += 64u) {
-        if (i >= base) {
+      for (uint32_t i = lane; i < (count > a.k ? count : a.k); i += 64u) {
+        if (i >= count) {
           write_nothing(a, row, i);
           continue;
         }
         const uint64_t mine = list[i];
         uint32_t rank = 0u;
-        for (uint32_t j = 0; j < base; ++j) rank += list[j] > mine;
-        write_candidate(a, row, rank, mine);
+        for (uint32_t j = 0; j < count; ++j) rank += list[j] > mine;
+        if (rank < a.k) write_candidate(a, row, rank, mine);
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();  // the next row's candidates go into the same list
@@ -489,7 +605,7 @@ __global__ __launch_bounds__(NT) void top_block_kernel(const TopArgs a) {
   uint32_t* ctl = reinterpret_cast<uint32_t*>(part + 2 * kWaves);  // [0] bound, [1] candidates, [2 ..] counts per wave
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
   const uint32_t packs = (a.K + N - 1u) / N;
-  const float c2 = (float)(1.4426950408889634 / a.temperature);
+  const float c2 = (float)(kLog2e / a.temperature);
   for (uint64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
     const T* in = static_cast<const T*>(a.in) + row * a.stride;
     ExpSum e;
@@ -618,17 +734,6 @@ __global__ __launch_bounds__(NT) void top_block_kernel(const TopArgs a) {
 // The sums are kept apart because 1 - sum_S p and a loss near zero are differences of near numbers: p_R comes from its own sum, and an
 // error of s_o moves all p together so that it enters the loss times (p_R - q_R) only.
 // ---------------------------------------------------------------------------------------------------
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
-  return v;
-}
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) v = fmaxf(v, __shfl_xor(v, d));
-  return v;
-}
-
 // what the gradient's pass over the row needs: grad = coef * exp((x - m) / T) outside S
 struct RowGrad {
   float m, coef;
@@ -650,7 +755,7 @@ struct Entries {
 // one wave, one row: the teacher's entries against the student's row.  o = sums outside S.
 template <class T, bool GRAD>
 __device__ __forceinline__ RowGrad row_loss(const DistillArgs& a, uint64_t row, const Entries& en, uint32_t lane, const ExpSum& o) {
-  const double inv_T = 1.0 / a.temperature;
+  const double inv_T = 1.0 / a.temperature, inv_T2 = inv_T * kLog2e;
   float xm = -FLT_MAX, tm = -FLT_MAX;
   for (uint32_t j = lane; j < a.k; j += 64u)
     if (en.id[j] >= 0) xm = fmaxf(xm, en.x[j]), tm = fmaxf(tm, en.t[j]);
@@ -660,15 +765,15 @@ __device__ __forceinline__ RowGrad row_loss(const DistillArgs& a, uint64_t row, 
   double zs = 0.0, ts = 0.0;
   for (uint32_t j = lane; j < a.k; j += 64u)
     if (en.id[j] >= 0) {
-      const double e = exp(((double)en.x[j] - (double)M) * inv_T), q = exp((double)en.t[j] * inv_T - shift);
+      const double e = exp2_64(((double)en.x[j] - (double)M) * inv_T2), q = exp2_64(((double)en.t[j] * inv_T - shift) * kLog2e);
       en.e[j] = e, en.q[j] = q;
       ts += q;
       if (!(en.id[j] & kAgain)) zs += e;
     }
   zs = wave_sum(zs), ts = wave_sum(ts);
-  const double far = exp(((double)o.m - (double)M) * inv_T), Z = (double)o.s * far + zs, log_Z = log(Z);
+  const double far = exp2_64(((double)o.m - (double)M) * inv_T2), Z = (double)o.s * far + zs, log_Z = log_64(Z);
   // without lse the q are still to be divided by their sum
-  const double log_T = a.lse ? shift : shift + log(ts), scale = a.lse ? 1.0 : 1.0 / ts;
+  const double log_T = a.lse ? shift : shift + log_64(ts), scale = a.lse ? 1.0 : 1.0 / ts;
   double Q = a.lse ? ts : 1.0, rest = 0.0, loss = 0.0;
   for (uint32_t j = lane; j < a.k; j += 64u)
     if (en.id[j] >= 0 && !(en.q[j] == 0.0))
@@ -676,7 +781,7 @@ __device__ __forceinline__ RowGrad row_loss(const DistillArgs& a, uint64_t row, 
   loss = wave_sum(loss);
   if (a.lse && o.s > 0.f && Q < 1.0) {
     rest = 1.0 - Q;
-    loss += rest * (log(rest) - (((double)o.m - (double)M) * inv_T + log((double)o.s) - log_Z));
+    loss += rest * (log_64(rest) - (((double)o.m - (double)M) * inv_T + log_64((double)o.s) - log_Z));
     Q = 1.0;
   }
   if (a.loss && lane == 0u) a.loss[row] = (float)loss;
@@ -715,7 +820,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void distill_kernel(const Dist
   float* part = reinterpret_cast<float*>(ctl + 4);       // [2 * kWaves]
   uint32_t* bitmap = ctl + 4 + 2u * kWaves;              // [words]
   const uint32_t packs = (a.K + N - 1u) / N;
-  const float c2 = (float)(1.4426950408889634 / a.temperature);
+  const float c2 = (float)(kLog2e / a.temperature);
   auto sync = [] {
     if (NT == 64) {
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -812,8 +917,8 @@ __global__ __launch_bounds__(256) void distill_thread_kernel(const DistillArgs a
   T* stage = reinterpret_cast<T*>(lds_words);
   const uint32_t pitch = staged_pitch<T>(a.K), gpitch = a.K | 1u;
   float* gstage = reinterpret_cast<float*>(lds_words + (256u * pitch * sizeof(T)) / 4u);
-  const double inv_T = 1.0 / a.temperature;
-  const float c2 = (float)(1.4426950408889634 / a.temperature);
+  const double inv_T = 1.0 / a.temperature, inv_T2 = inv_T * kLog2e;
+  const float c2 = (float)(kLog2e / a.temperature);
   for (uint64_t r0 = (uint64_t)blockIdx.x * 256u; r0 < a.n; r0 += (uint64_t)gridDim.x * 256u) {
     const uint32_t rows = (uint32_t)(a.n - r0 < 256u ? a.n - r0 : 256u);
     __syncthreads();
@@ -845,19 +950,19 @@ __global__ __launch_bounds__(256) void distill_thread_kernel(const DistillArgs a
         double zs = 0.0;
         for (uint32_t c = 0; c < a.K; ++c) {
           const float v = (float)x[c];
-          if ((listed >> c) & 1u) zs += exp(((double)v - (double)M) * inv_T);
+          if ((listed >> c) & 1u) zs += exp2_64(((double)v - (double)M) * inv_T2);
           else os += exp2_fast((v - om) * c2);
         }
-        const double far = exp(((double)om - (double)M) * inv_T), Z = (double)os * far + zs, log_Z = log(Z);
-        const double lse = a.lse ? (double)a.lse[row] : 0.0;
+        const double far = exp2_64(((double)om - (double)M) * inv_T2), Z = (double)os * far + zs, log_Z = log_64(Z);
+        const double shift = a.lse ? (double)a.lse[row] : (double)tm * inv_T;
         double ts = 0.0;
         for (uint32_t j = 0; j < a.k; ++j)
-          if ((uint32_t)ids[j] < a.K) ts += a.lse ? exp((double)tv[j] * inv_T - lse) : exp(((double)tv[j] - (double)tm) * inv_T);
-        const double log_T = a.lse ? lse : (double)tm * inv_T + log(ts);
+          if ((uint32_t)ids[j] < a.K) ts += exp2_64(((double)tv[j] * inv_T - shift) * kLog2e);
+        const double log_T = a.lse ? shift : shift + log_64(ts);
         double Q = a.lse ? ts : 1.0, rest = 0.0, loss = 0.0;
         if (a.lse && os > 0.f && Q < 1.0) {
           rest = 1.0 - Q;
-          loss = rest * (log(rest) - (((double)om - (double)M) * inv_T + log((double)os) - log_Z));
+          loss = rest * (log_64(rest) - (((double)om - (double)M) * inv_T + log_64((double)os) - log_Z));
           Q = 1.0;
         }
         const double w = GRAD ? (a.weight ? (double)a.weight[row * a.weight_stride] : 1.0) * inv_T : 0.0;
@@ -871,15 +976,15 @@ __global__ __launch_bounds__(256) void distill_thread_kernel(const DistillArgs a
         for (uint32_t j = 0; j < a.k; ++j)
           if ((uint32_t)ids[j] < a.K) {
             const uint32_t c = (uint32_t)ids[j];
-            const double lq = (double)tv[j] * inv_T - log_T, q = exp(lq), z = ((double)(float)x[c] - (double)M) * inv_T;
+            const double lq = (double)tv[j] * inv_T - log_T, q = exp2_64(lq * kLog2e), z = ((double)(float)x[c] - (double)M) * inv_T;
             if (!(q == 0.0)) loss += q * (lq - (z - log_Z));
             if (GRAD && ((open >> c) & 1u)) {
               open &= ~(1u << c);
               double qc = q;
               if (repeats)
                 for (uint32_t i = j + 1u; i < a.k; ++i)
-                  if (ids[i] == (int32_t)c) qc += exp((double)tv[i] * inv_T - log_T);
-              g[c] = (float)((exp(z) / Z * Q - qc) * w);
+                  if (ids[i] == (int32_t)c) qc += exp2_64(((double)tv[i] * inv_T - log_T) * kLog2e);
+              g[c] = (float)((exp2_64(z * kLog2e) / Z * Q - qc) * w);
             }
           }
         if (a.loss) a.loss[row] = (float)loss;
@@ -963,7 +1068,7 @@ template <class T, bool CM>
 hipError_t top_wave(const TopArgs& a, hipStream_t s) {
   constexpr uint32_t N = Pack<T>::N, rows = top_wave_rows(CM), threads = top_wave_waves(CM) * 64u;
   const uint64_t blocks = (a.n + rows - 1) / rows;
-  const uint32_t lds = top_wave_waves(CM) * a.k * 8u + (CM ? a.K * 16u * (uint32_t)sizeof(T) : 0u), packs = (a.K + N - 1) / N;
+  const uint32_t lds = top_wave_waves(CM) * wave_list(a.k) * 8u + (CM ? a.K * 16u * (uint32_t)sizeof(T) : 0u), packs = (a.K + N - 1) / N;
   if (packs <= 64u) return launch(top_wave_kernel<T, CM, 1>, blocks, threads, lds, s, a);
   if (packs <= 128u) return launch(top_wave_kernel<T, CM, 2>, blocks, threads, lds, s, a);
   if (packs <= 256u) return launch(top_wave_kernel<T, CM, 4>, blocks, threads, lds, s, a);
