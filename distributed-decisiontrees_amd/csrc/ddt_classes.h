@@ -46,6 +46,7 @@ struct DistillArgs {
   float* loss;  // may be NULL with a gradient
   void* grad;   // NULL = loss only
   uint64_t grad_stride;
+  bool past_caches;  // set by launch_distill
 };
 
 constexpr uint32_t kTopMaxClassMajor = 2048;  // classes of a class-major matrix that the wave-per-row kernel stages in LDS

@@ -40,20 +40,69 @@ __device__ __forceinline__ void load_pack(const T* row, uint32_t c, uint32_t end
     for (uint32_t i = 0; i < N; ++i) x[i] = c + i < end ? (float)row[c + i] : fill;
   }
 }
-template <class T>
+// four whole packs, STEP packs apart
+template <class T, uint32_t STEP>
+__device__ __forceinline__ void load_packs(const T* row, uint32_t p, float (&x)[4 * Pack<T>::N]) {
+  constexpr uint32_t N = Pack<T>::N;
+  typename Pack<T>::vec v[4];
+#pragma unroll
+  for (uint32_t u = 0; u < 4; ++u) __builtin_memcpy(&v[u], row + (size_t)(p + u * STEP) * N, 16);
+#pragma unroll
+  for (uint32_t u = 0; u < 4; ++u)
+#pragma unroll
+    for (uint32_t i = 0; i < N; ++i) x[u * N + i] = (float)v[u][i];
+}
+// PAST: nontemporal, so that what is written does not push out what will be read again
+template <class T, bool PAST = false>
 __device__ __forceinline__ void store_pack(T* row, uint32_t c, uint32_t end, const float (&x)[Pack<T>::N]) {
   constexpr uint32_t N = Pack<T>::N;
   if (c + N <= end) {
     typename Pack<T>::vec v;
 #pragma unroll
     for (uint32_t i = 0; i < N; ++i) v[i] = (T)x[i];
-    __builtin_memcpy(row + c, &v, 16);
+    typedef typename Pack<T>::vec anywhere __attribute__((aligned(sizeof(T))));
+    if (PAST) __builtin_nontemporal_store(v, reinterpret_cast<anywhere*>(row + c));
+    else __builtin_memcpy(row + c, &v, 16);
   } else {
 #pragma unroll
     for (uint32_t i = 0; i < N; ++i)
       if (c + i < end) row[c + i] = (T)x[i];
   }
 }
+
+// A pack kept in registers as it came.  hold() ends what the compiler may carry over from one use to the next: without it the fp32
+// forms of all packs stay live beside the packs themselves, twice the registers.
+template <class T>
+struct HeldPack {
+  static constexpr uint32_t N = Pack<T>::N;
+  uint32_t w[4];
+  __device__ __forceinline__ void load(const T* row, uint32_t c, uint32_t end) {
+    if (c + N <= end) {
+      __builtin_memcpy(w, row + c, 16);
+    } else {
+      typename Pack<T>::vec v;
+#pragma unroll
+      for (uint32_t i = 0; i < N; ++i) v[i] = c + i < end ? row[c + i] : (T)-kInf;
+      __builtin_memcpy(w, &v, 16);
+    }
+  }
+  __device__ __forceinline__ void get(float (&x)[N]) const {
+    typename Pack<T>::vec v;
+    __builtin_memcpy(&v, w, 16);
+#pragma unroll
+    for (uint32_t i = 0; i < N; ++i) x[i] = (float)v[i];
+  }
+  __device__ __forceinline__ void clear(uint32_t bits) {  // -inf where a bit is set
+    typename Pack<T>::vec v;
+    __builtin_memcpy(&v, w, 16);
+#pragma unroll
+    for (uint32_t i = 0; i < N; ++i) v[i] = (bits >> i) & 1u ? (T)-kInf : v[i];
+    __builtin_memcpy(w, &v, 16);
+  }
+  __device__ __forceinline__ void hold() { asm volatile("" : "+v"(w[0]), "+v"(w[1]), "+v"(w[2]), "+v"(w[3])); }
+};
+
+__device__ __forceinline__ void forget(uint32_t& v) { asm volatile("" : "+v"(v)); }
 
 // x ^ 2: the hardware instruction (1 ulp; results below 2^-126 may come back as 0 -- nothing next to a sum whose largest term is 1)
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -341,6 +390,45 @@ struct ExpSum {
     m = M;
   }
 };
+// The same, one instruction per score less, for the long rows: exponentials of fma(x, c, -r) with r an fp32 number a step or two above
+// m c -- never below it, where 2^(m c - r) of a large score's rounding would overflow.  finish() puts the difference right.  Where that rounding is no longer small against 1 (a largest score beyond 10^6 T, or a row without any,
+// whose m is the lowest number) it asks for the sum in the plain form instead.
+constexpr float kPlainBeyond = 0x1p20f;
+struct RunSum {
+  float m = -FLT_MAX, r, s = 0.f;
+  __device__ __forceinline__ explicit RunSum(float c) : r(reference(-FLT_MAX, c)) {}
+  static __device__ __forceinline__ float reference(float m, float c) {
+    return fminf(fmaxf(fmaf(fabsf(m * c), 0x1p-23f, m * c), -FLT_MAX), FLT_MAX);
+  }
+  template <uint32_t M>
+  __device__ __forceinline__ void add(const float (&x)[M], float c) {
+    float pm = x[0];
+#pragma unroll
+    for (uint32_t i = 1; i < M; ++i) pm = fmaxf(pm, x[i]);
+    if (pm > m) {
+      const float nr = reference(pm, c);
+      s *= exp2_fast(r - nr);
+      m = pm, r = nr;
+    }
+    float t[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (uint32_t i = 0; i < M; ++i) t[i & 3u] += exp2_fast(fmaf(x[i], c, -r));
+    s += (t[0] + t[1]) + (t[2] + t[3]);
+  }
+  // over the wave; plain(M) = this lane's sum of exp2((x - M) c)
+  template <class Plain>
+  __device__ __forceinline__ ExpSum finish(float c, Plain plain) const {
+    ExpSum e;
+    e.m = wave_max(m);
+    if (fabsf(e.m * c) <= kPlainBeyond) {
+      const float R = reference(e.m, c);
+      e.s = wave_sum(s * exp2_fast(r - R)) * exp2_fast((float)fma((double)e.m, -(double)c, (double)R));
+    } else {
+      e.s = wave_sum(plain(e.m));
+    }
+    return e;
+  }
+};
 __device__ __forceinline__ float log_sum(const ExpSum& e, double inv_T) {
   if (e.m == kInf) return kInf;
   return (float)((double)e.m * inv_T + log_64((double)e.s));  // nothing but -inf: log 0 = -inf
@@ -371,7 +459,7 @@ __device__ __forceinline__ void write_nothing(const TopArgs& a, uint64_t row, ui
   a.values[row * a.k + rank] = -kInf;
 }
 
-// few classes, few of them wanted: a thread per row, the best KK in registers.  Row-major rows are staged in LDS (coalesced loads;
+// few classes, few of them wanted: a thread per row, the best k = KK in registers.  Row-major rows are staged in LDS (coalesced loads;
 // the row pitch is an odd number of words), class-major ones are coalesced as they are.
 template <class T>
 __device__ __forceinline__ uint32_t staged_pitch(uint32_t K) {  // elements
@@ -442,9 +530,8 @@ __global__ __launch_bounds__(256) void top_thread_kernel(const TopArgs a) {
         }
       }
     }
-#pragma unroll
-    for (int j = 0; j < KK; ++j)
-      if ((uint32_t)j < a.k) a.ids[row * a.k + j] = id[j], a.values[row * a.k + j] = v[j];
+    __builtin_memcpy(a.ids + row * KK, id, sizeof(id));  // (one store: a wave writes one piece)
+    __builtin_memcpy(a.values + row * KK, v, sizeof(v));
     if (a.lse) a.lse[row] = log_sum(e, 1.0 / a.temperature);
   }
 }
@@ -602,27 +689,39 @@ __global__ __launch_bounds__(NT) void top_block_kernel(const TopArgs a) {
   uint64_t* list = reinterpret_cast<uint64_t*>(lds_words);         // [kListCap]
   uint32_t* maxima = lds_words + 2 * kListCap;                     // [NT]
   float* part = reinterpret_cast<float*>(maxima + NT);             // [2 * kWaves]
-  uint32_t* ctl = reinterpret_cast<uint32_t*>(part + 2 * kWaves);  // [0] bound, [1] candidates, [2 ..] counts per wave
+  uint32_t* ctl = reinterpret_cast<uint32_t*>(part + 2 * kWaves);  // [0] bound, [1] candidates, [2] threads that hold them, [3 ..] counts per wave
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
   const uint32_t packs = (a.K + N - 1u) / N;
   const float c2 = (float)(kLog2e / a.temperature);
   for (uint64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
     const T* in = static_cast<const T*>(a.in) + row * a.stride;
-    ExpSum e;
-    float top = -kInf;
-    for (uint32_t p = tid; p < packs; p += NT) {
+    RunSum run(c2);
+    uint32_t p0 = 0;
+    for (; (p0 + 4u * NT) * N <= a.K; p0 += 4u * NT) {  // four packs of a thread in flight
+      float x[4 * N];
+      load_packs<T, NT>(in, p0 + tid, x);
+      run.add(x, c2);
+    }
+    for (uint32_t p = p0 + tid; p < packs; p += NT) {
       float x[N];
       load_pack(in, p * N, a.K, -kInf, x);
-      e.add(x, c2);
-#pragma unroll
-      for (uint32_t i = 0; i < N; ++i) top = fmaxf(top, x[i]);
+      run.add(x, c2);
     }
-    const uint32_t best = score_key(top);
-    e.reduce_wave(c2);
+    const uint32_t best = score_key(run.m);  // (a thread without a candidate counts with the lowest score: the bound only sinks)
+    const ExpSum e = run.finish(c2, [&](float M) {
+      float t = 0.f;
+      for (uint32_t p = tid; p < packs; p += NT) {
+        float x[N];
+        load_pack(in, p * N, a.K, -kInf, x);
+#pragma unroll
+        for (uint32_t i = 0; i < N; ++i) t += exp2_fast((x[i] - M) * c2);
+      }
+      return t;
+    });
     __syncthreads();  // the row before is written
     maxima[tid] = best;
     if (lane == 0u) part[2 * wave] = e.m, part[2 * wave + 1] = e.s;
-    if (tid == 0u) ctl[1] = 0u;
+    if (tid == 0u) ctl[1] = 0u, ctl[2] = 0u;
     __syncthreads();
     if (wave == 0u) {
       constexpr int E = NT / 64;
@@ -640,19 +739,33 @@ __global__ __launch_bounds__(NT) void top_block_kernel(const TopArgs a) {
     __syncthreads();
     const uint32_t bound = ctl[0];
     const bool mine = best >= bound;
-    if (mine)
-      for (uint32_t p = tid; p < packs; p += NT) {
-        float x[N];
-        load_pack(in, p * N, a.K, -kInf, x);
+    uint32_t* owners = maxima;  // threads whose packs hold candidates
+    if (mine) owners[atomicAdd(&ctl[2], 1u)] = tid;
+    __syncthreads();
+    {
+      // their packs, dealt out over the whole block: item i = pack (i mod per) of owner (i div per)
+      const uint32_t per = (packs + NT - 1u) / NT, items = ctl[2] * per, magic = 0xFFFFFFFFu / per + 1u;  // (i per < 2^32; per = 1: magic 0)
+      for (uint32_t i0 = tid; i0 < items; i0 += 4u * NT) {
+        float x[4][N];
+        uint32_t c[4];
 #pragma unroll
-        for (uint32_t i = 0; i < N; ++i) {
-          const uint32_t key = score_key(x[i]);
-          if (key >= bound) {
-            const uint32_t slot = atomicAdd(&ctl[1], 1u);
-            if (slot < kListCap) list[slot] = candidate(key, p * N + i);
-          }
+        for (uint32_t u = 0; u < 4; ++u) {
+          const uint32_t i = i0 + u * NT, o = per == 1u ? i : __umulhi(i, magic);
+          c[u] = i < items ? (owners[o] + (i - o * per) * NT) * N : a.K;
+          load_pack(in, c[u], a.K, -kInf, x[u]);
         }
+#pragma unroll
+        for (uint32_t u = 0; u < 4; ++u)
+#pragma unroll
+          for (uint32_t j = 0; j < N; ++j) {
+            const uint32_t key = score_key(x[u][j]);
+            if (key >= bound) {
+              const uint32_t slot = atomicAdd(&ctl[1], 1u);
+              if (slot < kListCap) list[slot] = candidate(key, c[u] + j);
+            }
+          }
       }
+    }
     __syncthreads();
     uint32_t count = ctl[1];
     if (count > kListCap) {
@@ -673,10 +786,10 @@ __global__ __launch_bounds__(NT) void top_block_kernel(const TopArgs a) {
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) n += __shfl_xor(n, d);
         __syncthreads();
-        if (lane == 0u) ctl[2 + wave] = n;
+        if (lane == 0u) ctl[3 + wave] = n;
         __syncthreads();
         uint32_t sum = 0u;
-        for (uint32_t w = 0; w < kWaves; ++w) sum += ctl[2 + w];
+        for (uint32_t w = 0; w < kWaves; ++w) sum += ctl[3 + w];
         return sum;
       };
       uint32_t t = bound;  // raised to the kk-th largest key: bits below the bound's differing ones are tried from the top
@@ -755,7 +868,9 @@ struct Entries {
 // one wave, one row: the teacher's entries against the student's row.  o = sums outside S.
 template <class T, bool GRAD>
 __device__ __forceinline__ RowGrad row_loss(const DistillArgs& a, uint64_t row, const Entries& en, uint32_t lane, const ExpSum& o) {
-  const double inv_T = 1.0 / a.temperature, inv_T2 = inv_T * kLog2e;
+  // the student's scale is the fp32 one of the sums outside S, for all its classes: p stays a softmax, of a temperature off by 2^-25
+  const double inv_T = 1.0 / a.temperature, x_scale = (double)(float)(kLog2e / a.temperature);
+  constexpr double kLn2 = 0.69314718055994530942;
   float xm = -FLT_MAX, tm = -FLT_MAX;
   for (uint32_t j = lane; j < a.k; j += 64u)
     if (en.id[j] >= 0) xm = fmaxf(xm, en.x[j]), tm = fmaxf(tm, en.t[j]);
@@ -765,23 +880,23 @@ __device__ __forceinline__ RowGrad row_loss(const DistillArgs& a, uint64_t row, 
   double zs = 0.0, ts = 0.0;
   for (uint32_t j = lane; j < a.k; j += 64u)
     if (en.id[j] >= 0) {
-      const double e = exp2_64(((double)en.x[j] - (double)M) * inv_T2), q = exp2_64(((double)en.t[j] * inv_T - shift) * kLog2e);
+      const double e = exp2_64(((double)en.x[j] - (double)M) * x_scale), q = exp2_64(((double)en.t[j] * inv_T - shift) * kLog2e);
       en.e[j] = e, en.q[j] = q;
       ts += q;
       if (!(en.id[j] & kAgain)) zs += e;
     }
   zs = wave_sum(zs), ts = wave_sum(ts);
-  const double far = exp2_64(((double)o.m - (double)M) * inv_T2), Z = (double)o.s * far + zs, log_Z = log_64(Z);
+  const double far = exp2_64(((double)o.m - (double)M) * x_scale), Z = (double)o.s * far + zs, log_Z = log_64(Z);
   // without lse the q are still to be divided by their sum
   const double log_T = a.lse ? shift : shift + log_64(ts), scale = a.lse ? 1.0 : 1.0 / ts;
   double Q = a.lse ? ts : 1.0, rest = 0.0, loss = 0.0;
   for (uint32_t j = lane; j < a.k; j += 64u)
     if (en.id[j] >= 0 && !(en.q[j] == 0.0))
-      loss += en.q[j] * scale * (((double)en.t[j] * inv_T - log_T) - (((double)en.x[j] - (double)M) * inv_T - log_Z));
+      loss += en.q[j] * scale * (((double)en.t[j] * inv_T - log_T) - (((double)en.x[j] - (double)M) * x_scale * kLn2 - log_Z));
   loss = wave_sum(loss);
   if (a.lse && o.s > 0.f && Q < 1.0) {
     rest = 1.0 - Q;
-    loss += rest * (log_64(rest) - (((double)o.m - (double)M) * inv_T + log_64((double)o.s) - log_Z));
+    loss += rest * (log_64(rest) - (((double)o.m - (double)M) * x_scale * kLn2 + log_64((double)o.s) - log_Z));
     Q = 1.0;
   }
   if (a.loss && lane == 0u) a.loss[row] = (float)loss;
@@ -807,11 +922,13 @@ __host__ __device__ constexpr uint32_t distill_words(uint32_t K, uint32_t k, uin
   return (Entries::words(k) + 4u + 2u * (threads / 64u) + (K + 31u) / 32u + 1u) & ~1u;
 }
 
-// NT threads per row: 64 (a wave; 4 rows per block of 256) or the whole block.  The row is read once for the sums outside S -- S as a
-// bitmap in LDS, a pack's bits next to each other -- and, for the gradient, a second time, from whichever cache still holds it.
-template <class T, int NT, bool GRAD>
+// NT threads per row: 64 (a wave; 4 rows per block of 256) or the whole block.  P > 0: the row's packs stay in registers, P per thread,
+// all of them loaded at once while the teacher's entries are fetched, so that the gradient costs one read and one write of the matrix.
+// P = 0 (rows of more than 512 x 32 packs): the row is read a second time for the gradient, from whichever cache still holds it.
+// S is a bitmap in LDS, a pack's bits next to each other.
+template <class T, int NT, int P, bool GRAD>
 __global__ __launch_bounds__(NT == 64 ? 256 : NT) void distill_kernel(const DistillArgs a) {
-  constexpr uint32_t N = Pack<T>::N, kGroups = NT == 64 ? 4 : 1, kWaves = NT / 64;
+  constexpr uint32_t N = Pack<T>::N, kGroups = NT == 64 ? 4 : 1, kWaves = NT / 64, kFull = (1u << N) - 1u;
   const uint32_t lane = threadIdx.x & 63u, group = NT == 64 ? threadIdx.x >> 6 : 0u, tid = NT == 64 ? lane : threadIdx.x;
   const uint32_t words = (a.K + 31u) / 32u;
   uint32_t* base = lds_words + group * distill_words(a.K, a.k, NT);
@@ -829,21 +946,41 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void distill_kernel(const Dist
       __syncthreads();
     }
   };
+  auto listed_bits = [&](uint32_t p) { return bitmap[p * N >> 5] >> (p * N & 31u) & kFull; };
   for (uint64_t row = (uint64_t)blockIdx.x * kGroups + group; row < a.n; row += (uint64_t)gridDim.x * kGroups) {
     const T* in = static_cast<const T*>(a.in) + row * a.stride;
     T* out = static_cast<T*>(a.grad) + row * a.grad_stride;
     sync();  // the row before is done with the LDS
     for (uint32_t i = tid; i < words; i += NT) bitmap[i] = 0u;
     if (tid < 2u) ctl[tid] = 0u;
+    // a block's thread fetches one entry and its score of the student itself: ahead of the row, which the score is read behind
+    static_assert(NT == 64 || NT >= DDT_MAX_TOP, "an entry per thread");
+    int32_t my_id = -1;
+    float my_t = 0.f, my_x = 0.f;
+    if (NT > 64 && tid < a.k) my_id = a.ids[row * a.teacher_stride + tid], my_t = a.values[row * a.teacher_stride + tid];
+    HeldPack<T> raw[P > 0 ? P : 1];
+    uint32_t own = tid;  // the thread's first pack; opaque, so that the packs' indexes and addresses are computed where they are used
+    forget(own);
+#pragma unroll
+    for (int i = 0; i < P; ++i) raw[i].load(in, (own + (uint32_t)i * NT) * N, a.K);
     sync();
-    for (uint32_t j = tid; j < a.k; j += NT) {
-      int32_t id = a.ids[row * a.teacher_stride + j];
-      if ((uint32_t)id >= a.K) id = -1;
-      en.id[j] = id;
+    auto enter = [&](uint32_t j, int32_t id, float t) {
+      en.id[j] = id, en.t[j] = t;
       if (id >= 0) {
-        en.t[j] = a.values[row * a.teacher_stride + j], en.x[j] = (float)in[id];
         ctl[0] = 1u;
         if (atomicOr(&bitmap[id >> 5], 1u << (id & 31)) >> (id & 31) & 1u) ctl[1] = 1u;
+      }
+    };
+    if (NT > 64) {
+      if ((uint32_t)my_id >= a.K) my_id = -1;
+      if (tid < a.k) enter(tid, my_id, my_t);
+      if (my_id >= 0) my_x = (float)in[my_id];
+    } else {
+      for (uint32_t j = tid; j < a.k; j += NT) {
+        int32_t id = a.ids[row * a.teacher_stride + j];
+        if ((uint32_t)id >= a.K) id = -1;
+        enter(j, id, a.values[row * a.teacher_stride + j]);
+        if (id >= 0) en.x[j] = (float)in[id];
       }
     }
     sync();
@@ -866,18 +1003,63 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void distill_kernel(const Dist
         sync();
       }
     }
-    ExpSum o;
-    for (uint32_t p = tid; p < packs; p += NT) {
-      float x[N];
-      load_pack(in, p * N, a.K, -kInf, x);
-      const uint32_t bits = bitmap[p * N >> 5] >> (p * N & 31u);
-      if (bits & ((1u << N) - 1u)) {
+    RunSum run(c2);
+    uint32_t holds = 0u;  // packs (of the registers) that hold a listed class
+    if (P > 0) {
+      constexpr int C = P < 4 ? P : 4;  // packs that are summed at a time
+#pragma unroll
+      for (int i = 0; i < P; i += C) {
+        forget(own);
+        float x[(P > 0 ? C : 1) * N];
+#pragma unroll
+        for (int u = 0; u < C; ++u) {
+          const uint32_t p = own + (uint32_t)(i + u) * NT, bits = p < packs ? listed_bits(p) : 0u;
+          if (bits) holds |= 1u << (i + u), raw[i + u].clear(bits);
+          float v[N];
+          raw[i + u].get(v);
+#pragma unroll
+          for (uint32_t j = 0; j < N; ++j) x[u * N + j] = v[j];
+        }
+        if (own + (uint32_t)i * NT < packs) run.add(x, c2);
+#pragma unroll
+        for (int u = 0; u < C; ++u) raw[i + u].hold();
+      }
+    } else {
+      uint32_t p0 = 0;
+      for (; (p0 + 4u * NT) * N <= a.K; p0 += 4u * NT) {  // four packs of a thread in flight
+        float x[4 * N];
+        load_packs<T, NT>(in, p0 + tid, x);
+#pragma unroll
+        for (uint32_t u = 0; u < 4; ++u) {
+          const uint32_t bits = listed_bits(p0 + tid + u * NT);
+          if (bits) {
+#pragma unroll
+            for (uint32_t i = 0; i < N; ++i) x[u * N + i] = (bits >> i) & 1u ? -kInf : x[u * N + i];
+          }
+        }
+        run.add(x, c2);
+      }
+      for (uint32_t p = p0 + tid; p < packs; p += NT) {
+        float x[N];
+        load_pack(in, p * N, a.K, -kInf, x);
+        const uint32_t bits = listed_bits(p);
 #pragma unroll
         for (uint32_t i = 0; i < N; ++i) x[i] = (bits >> i) & 1u ? -kInf : x[i];
+        run.add(x, c2);
       }
-      o.add(x, c2);
     }
-    o.reduce_wave(c2);
+    ExpSum o = run.finish(c2, [&](float M) {
+      float t = 0.f;
+      for (uint32_t p = tid; p < packs; p += NT) {
+        float x[N];
+        load_pack(in, p * N, a.K, -kInf, x);
+        const uint32_t bits = listed_bits(p);
+#pragma unroll
+        for (uint32_t i = 0; i < N; ++i) t += (bits >> i) & 1u ? 0.f : exp2_fast((x[i] - M) * c2);
+      }
+      return t;
+    });
+    if (NT > 64 && tid < a.k) en.x[tid] = my_x;
     if (NT > 64) {
       if (lane == 0u) part[2 * (tid >> 6)] = o.m, part[2 * (tid >> 6) + 1] = o.s;
       sync();
@@ -893,100 +1075,163 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void distill_kernel(const Dist
     if (GRAD) {
       sync();
       const float m = __uint_as_float(ctl[2]), coef = __uint_as_float(ctl[3]);
-      for (uint32_t p = tid; p < packs; p += NT) {
-        float x[N];
-        load_pack(in, p * N, a.K, -kInf, x);
-        const uint32_t bits = bitmap[p * N >> 5] >> (p * N & 31u);
-#pragma unroll
-        for (uint32_t i = 0; i < N; ++i) x[i] = coef * exp2_fast((x[i] - m) * c2);
-        if (bits & ((1u << N) - 1u)) {  // the listed classes of this pack are written already
+      auto write = [&](uint32_t p, const float (&x)[N], bool check) {
+        const uint32_t bits = check ? listed_bits(p) : 0u;
+        if (bits) {  // the listed classes of this pack are written already
 #pragma unroll
           for (uint32_t i = 0; i < N; ++i)
             if (p * N + i < a.K && !((bits >> i) & 1u)) out[p * N + i] = (T)x[i];
+        } else if (a.past_caches) {
+          store_pack<T, true>(out, p * N, a.K, x);
         } else {
-          store_pack(out, p * N, a.K, x);
+          store_pack<T>(out, p * N, a.K, x);
+        }
+      };
+      // Two-byte gradients: coef goes into the exponent, with its sign put on afterwards -- two instructions per score less.  Its
+      // rounding there is below 2^-16 for |m c| up to 256, next to a result that is rounded to 11 bits at most.
+      const float b = log2f(fabsf(coef)) - m * c2;
+      const uint32_t sign = __float_as_uint(coef) & 0x80000000u;
+      const bool folded = sizeof(T) == 2 && fabsf(m * c2) <= 256.f;
+      auto plain = [&](float x) { return coef * exp2_fast((x - m) * c2); };
+      auto in_exponent = [&](float x) { return __uint_as_float(__float_as_uint(exp2_fast(fmaf(x, c2, b))) ^ sign); };
+      if (P > 0 && (sizeof(T) == 4 || folded)) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          forget(own);
+          if (own + (uint32_t)i * NT < packs) {
+            float x[N];
+            raw[i].get(x);
+#pragma unroll
+            for (uint32_t j = 0; j < N; ++j) x[j] = sizeof(T) == 4 ? plain(x[j]) : in_exponent(x[j]);
+            write(own + (uint32_t)i * NT, x, (holds >> i) & 1u);
+          }
+        }
+      } else {
+        // from the row's end, which was read last and is the likeliest to be in the L2 still; four packs of a thread in flight
+        const uint32_t whole = P == 0 && (sizeof(T) == 4 || folded) ? a.K / (4u * NT * N) * (4u * NT) : 0u;
+        if (P == 0)
+          for (uint32_t p0 = whole; p0 > 0u;) {
+            p0 -= 4u * NT;
+            float x[4 * N];
+            load_packs<T, NT>(in, p0 + tid, x);
+#pragma unroll
+            for (uint32_t u = 0; u < 4; ++u) {
+              float y[N];
+#pragma unroll
+              for (uint32_t j = 0; j < N; ++j) y[j] = sizeof(T) == 4 ? plain(x[u * N + j]) : in_exponent(x[u * N + j]);
+              write(p0 + tid + u * NT, y, true);
+            }
+          }
+        for (uint32_t p = whole + tid; p < packs; p += NT) {
+          float x[N];
+          load_pack(in, p * N, a.K, -kInf, x);
+#pragma unroll
+          for (uint32_t j = 0; j < N; ++j) x[j] = plain(x[j]);
+          write(p, x, true);
         }
       }
     }
   }
 }
 
-// up to 32 classes: a thread per row, rows staged in LDS and their gradients collected there in fp32
-template <class T, bool GRAD>
+// up to 32 classes: a thread per row, rows staged in LDS and their gradients collected there in fp32.  KK > 0: k = KK entries per row,
+// in registers with their exponentials; KK = 0: any number, read and computed again where they are needed.
+template <class T, int KK, bool GRAD>
 __global__ __launch_bounds__(256) void distill_thread_kernel(const DistillArgs a) {
   T* stage = reinterpret_cast<T*>(lds_words);
   const uint32_t pitch = staged_pitch<T>(a.K), gpitch = a.K | 1u;
   float* gstage = reinterpret_cast<float*>(lds_words + (256u * pitch * sizeof(T)) / 4u);
-  const double inv_T = 1.0 / a.temperature, inv_T2 = inv_T * kLog2e;
+  constexpr double kLn2 = 0.69314718055994530942;
   const float c2 = (float)(kLog2e / a.temperature);
+  const double inv_T = 1.0 / a.temperature, x_scale = (double)c2;
   for (uint64_t r0 = (uint64_t)blockIdx.x * 256u; r0 < a.n; r0 += (uint64_t)gridDim.x * 256u) {
     const uint32_t rows = (uint32_t)(a.n - r0 < 256u ? a.n - r0 : 256u);
+    const bool active = threadIdx.x < rows;
+    const uint64_t row = r0 + threadIdx.x;
+    const int32_t* ids = a.ids + row * a.teacher_stride;
+    const float* tv = a.values + row * a.teacher_stride;
+    int32_t id[KK > 0 ? KK : 1];
+    float t[KK > 0 ? KK : 1];
+    double eq[KK > 0 ? KK : 1][2];
+    float given_lse = 0.f, weight = 1.f;
+    if (active) {
+      if (KK > 0) __builtin_memcpy(id, ids, sizeof(id)), __builtin_memcpy(t, tv, sizeof(t));
+      if (a.lse) given_lse = a.lse[row];
+      if (GRAD && a.weight) weight = a.weight[row * a.weight_stride];
+    }
     __syncthreads();
     stage_rows(static_cast<const T*>(a.in), r0, rows, a.K, a.stride, stage, pitch);
     __syncthreads();
-    if (threadIdx.x < rows) {
-      const uint64_t row = r0 + threadIdx.x;
+    if (active) {
       const T* x = stage + threadIdx.x * pitch;
       float* g = gstage + threadIdx.x * gpitch;
-      const int32_t* ids = a.ids + row * a.teacher_stride;
-      const float* tv = a.values + row * a.teacher_stride;
+      auto each = [&](auto f) {  // f(entry, class, score) of the row's entries, in order
+        if constexpr (KK > 0) {
+#pragma unroll
+          for (int j = 0; j < KK; ++j)
+            if ((uint32_t)id[j] < a.K) f(j, (uint32_t)id[j], t[j]);
+        } else {
+          for (uint32_t j = 0; j < a.k; ++j)
+            if ((uint32_t)ids[j] < a.K) f(j, (uint32_t)ids[j], tv[j]);
+        }
+      };
       uint32_t listed = 0u, entries = 0u;
       float tm = -FLT_MAX;
-      for (uint32_t j = 0; j < a.k; ++j)
-        if ((uint32_t)ids[j] < a.K) listed |= 1u << ids[j], tm = fmaxf(tm, tv[j]), ++entries;
+      each([&](uint32_t, uint32_t c, float v) { listed |= 1u << c, tm = fmaxf(tm, v), ++entries; });
       if (listed == 0u) {
         if (a.loss) a.loss[row] = 0.f;
         if (GRAD)
           for (uint32_t c = 0; c < a.K; ++c) g[c] = 0.f;
       } else {
-        float om = -FLT_MAX, sm = -FLT_MAX;
+        float om = -FLT_MAX, sm = -FLT_MAX, os = 0.f;
         for (uint32_t c = 0; c < a.K; ++c) {
           const float v = (float)x[c];
           if ((listed >> c) & 1u) sm = fmaxf(sm, v);
           else om = fmaxf(om, v);
         }
+        for (uint32_t c = 0; c < a.K; ++c) os += (listed >> c) & 1u ? 0.f : exp2_fast(((float)x[c] - om) * c2);
         const float M = fmaxf(om, sm);
-        float os = 0.f;
-        double zs = 0.0;
-        for (uint32_t c = 0; c < a.K; ++c) {
-          const float v = (float)x[c];
-          if ((listed >> c) & 1u) zs += exp2_64(((double)v - (double)M) * inv_T2);
-          else os += exp2_fast((v - om) * c2);
-        }
-        const double far = exp2_64(((double)om - (double)M) * inv_T2), Z = (double)os * far + zs, log_Z = log_64(Z);
-        const double shift = a.lse ? (double)a.lse[row] : (double)tm * inv_T;
-        double ts = 0.0;
-        for (uint32_t j = 0; j < a.k; ++j)
-          if ((uint32_t)ids[j] < a.K) ts += exp2_64(((double)tv[j] * inv_T - shift) * kLog2e);
-        const double log_T = a.lse ? shift : shift + log_64(ts);
+        const double shift = a.lse ? (double)given_lse : (double)tm * inv_T;
+        auto student = [&](uint32_t c) { return ((double)(float)x[c] - (double)M) * x_scale; };
+        auto teacher = [&](float v) { return exp2_64(((double)v * inv_T - shift) * kLog2e); };
+        double zs = 0.0, ts = 0.0;
+        uint32_t open = listed;  // classes of the list that are still to come
+        each([&](uint32_t j, uint32_t c, float v) {
+          const double e = exp2_64(student(c)), q = teacher(v);
+          if (KK > 0) eq[KK > 0 ? j : 0][0] = e, eq[KK > 0 ? j : 0][1] = q;
+          zs += (open >> c) & 1u ? e : 0.0;
+          ts += q;
+          open &= ~(1u << c);
+        });
+        const double far = exp2_64(((double)om - (double)M) * x_scale), Z = (double)os * far + zs, log_Z = log_64(Z);
+        const double log_T = a.lse ? shift : shift + log_64(ts), scale = a.lse ? 1.0 : 1.0 / ts;
         double Q = a.lse ? ts : 1.0, rest = 0.0, loss = 0.0;
         if (a.lse && os > 0.f && Q < 1.0) {
           rest = 1.0 - Q;
-          loss = rest * (log_64(rest) - (((double)om - (double)M) * inv_T + log_64((double)os) - log_Z));
+          loss = rest * (log_64(rest) - (((double)om - (double)M) * x_scale * kLn2 + log_64((double)os) - log_Z));
           Q = 1.0;
         }
-        const double w = GRAD ? (a.weight ? (double)a.weight[row * a.weight_stride] : 1.0) * inv_T : 0.0;
+        const double w = (double)weight * inv_T, p_scale = Q / Z;
         if (GRAD) {
-          const float coef = !(os == 0.f) ? (float)((Q * far / Z - rest / (double)os) * w) : Z == 0.0 ? __builtin_nanf("") : 0.f;
+          // (nothing outside the list: no gradient there; nothing in the whole row: NaN, as its softmax)
+          const float coef = !(os == 0.f) ? (float)((p_scale * far - rest / (double)os) * w) : Z == 0.0 ? __builtin_nanf("") : 0.f;
           for (uint32_t c = 0; c < a.K; ++c)
             if (!((listed >> c) & 1u)) g[c] = coef * exp2_fast(((float)x[c] - om) * c2);
         }
         const bool repeats = entries != (uint32_t)__popc(listed);
-        uint32_t open = listed;  // classes of the list whose gradient is still to be written
-        for (uint32_t j = 0; j < a.k; ++j)
-          if ((uint32_t)ids[j] < a.K) {
-            const uint32_t c = (uint32_t)ids[j];
-            const double lq = (double)tv[j] * inv_T - log_T, q = exp2_64(lq * kLog2e), z = ((double)(float)x[c] - (double)M) * inv_T;
-            if (!(q == 0.0)) loss += q * (lq - (z - log_Z));
-            if (GRAD && ((open >> c) & 1u)) {
-              open &= ~(1u << c);
-              double qc = q;
-              if (repeats)
-                for (uint32_t i = j + 1u; i < a.k; ++i)
-                  if (ids[i] == (int32_t)c) qc += exp2_64(((double)tv[i] * inv_T - log_T) * kLog2e);
-              g[c] = (float)((exp2_64(z * kLog2e) / Z * Q - qc) * w);
-            }
+        open = listed;
+        each([&](uint32_t j, uint32_t c, float v) {
+          const double q = KK > 0 ? eq[KK > 0 ? j : 0][1] : teacher(v);
+          if (!(q == 0.0)) loss += q * scale * (((double)v * inv_T - log_T) - (student(c) * kLn2 - log_Z));
+          if (GRAD && ((open >> c) & 1u)) {
+            open &= ~(1u << c);
+            double qc = q;
+            if (repeats)  // further entries of this class, in their order
+              for (uint32_t i = j + 1u; i < a.k; ++i)
+                if (ids[i] == (int32_t)c) qc += teacher(tv[i]);
+            g[c] = (float)(((KK > 0 ? eq[KK > 0 ? j : 0][0] : exp2_64(student(c))) * p_scale - qc * scale) * w);
           }
+        });
         if (a.loss) a.loss[row] = (float)loss;
       }
     }
@@ -1005,7 +1250,8 @@ __global__ __launch_bounds__(256) void distill_thread_kernel(const DistillArgs a
             v[j] = i + j < total ? gstage[r * gpitch + c] : 0.f;
             if (++c == a.K) c = 0u, ++r;
           }
-          store_pack(dst, i, total, v);
+          if (a.past_caches) store_pack<T, true>(dst, i, total, v);
+          else store_pack<T>(dst, i, total, v);
         }
       } else {
         for (uint32_t r = threadIdx.x >> 5; r < rows; r += 8u)
@@ -1059,10 +1305,16 @@ template <class T, bool CM>
 hipError_t top_thread(const TopArgs& a, hipStream_t s) {
   const uint64_t blocks = (a.n + 255) / 256;
   const uint32_t lds = CM ? 0u : 256u * (uint32_t)sizeof(T) * ((((a.K + 4 / sizeof(T) - 1) / (4 / sizeof(T))) | 1u) * (uint32_t)(4 / sizeof(T)));
-  if (a.k == 1u) return launch(top_thread_kernel<T, CM, 1>, blocks, 256, lds, s, a);
-  if (a.k == 2u) return launch(top_thread_kernel<T, CM, 2>, blocks, 256, lds, s, a);
-  if (a.k <= 4u) return launch(top_thread_kernel<T, CM, 4>, blocks, 256, lds, s, a);
-  return launch(top_thread_kernel<T, CM, 8>, blocks, 256, lds, s, a);
+  switch (a.k) {
+    case 1: return launch(top_thread_kernel<T, CM, 1>, blocks, 256, lds, s, a);
+    case 2: return launch(top_thread_kernel<T, CM, 2>, blocks, 256, lds, s, a);
+    case 3: return launch(top_thread_kernel<T, CM, 3>, blocks, 256, lds, s, a);
+    case 4: return launch(top_thread_kernel<T, CM, 4>, blocks, 256, lds, s, a);
+    case 5: return launch(top_thread_kernel<T, CM, 5>, blocks, 256, lds, s, a);
+    case 6: return launch(top_thread_kernel<T, CM, 6>, blocks, 256, lds, s, a);
+    case 7: return launch(top_thread_kernel<T, CM, 7>, blocks, 256, lds, s, a);
+    default: return launch(top_thread_kernel<T, CM, 8>, blocks, 256, lds, s, a);
+  }
 }
 template <class T, bool CM>
 hipError_t top_wave(const TopArgs& a, hipStream_t s) {
@@ -1077,31 +1329,53 @@ hipError_t top_wave(const TopArgs& a, hipStream_t s) {
 }
 template <class T, int NT>
 hipError_t top_block(const TopArgs& a, hipStream_t s) {
-  return launch(top_block_kernel<T, NT>, a.n, NT, 8u * kListCap + 4u * NT + 8u * (NT / 64) + 4u * (2u + NT / 64), s, a);
+  return launch(top_block_kernel<T, NT>, a.n, NT, 8u * kListCap + 4u * NT + 8u * (NT / 64) + 4u * (3u + NT / 64), s, a);
 }
 template <class T>
 hipError_t top_typed(const TopArgs& a, bool class_major, hipStream_t s) {
   if (a.K <= 32u && a.k <= 8u) return class_major ? top_thread<T, true>(a, s) : top_thread<T, false>(a, s);
   if (class_major) return a.K <= kTopMaxClassMajor ? top_wave<T, true>(a, s) : hipErrorInvalidValue;
   if (a.K <= 2048u) return top_wave<T, false>(a, s);
-  return a.K <= 16384u ? top_block<T, 256>(a, s) : top_block<T, 1024>(a, s);
+  if (a.K <= 16384u) return top_block<T, 256>(a, s);
+  return a.n > 256u ? top_block<T, 512>(a, s) : top_block<T, 1024>(a, s);
 }
 
-template <class T, int NT, bool GRAD>
+template <class T, int NT, int P, bool GRAD>
 hipError_t distill_rows(const DistillArgs& a, hipStream_t s) {
   constexpr uint32_t groups = NT == 64 ? 4u : 1u;
   const uint32_t lds = groups * 4u * distill_words(a.K, a.k, NT);
-  return launch(distill_kernel<T, NT, GRAD>, (a.n + groups - 1) / groups, NT == 64 ? 256 : NT, lds, s, a);
+  return launch(distill_kernel<T, NT, P, GRAD>, (a.n + groups - 1) / groups, NT == 64 ? 256 : NT, lds, s, a);
 }
 template <class T, bool GRAD>
 hipError_t distill_typed(const DistillArgs& a, hipStream_t s) {
   constexpr uint32_t per_word = 4 / sizeof(T);
   if (a.K <= 32u) {
     const uint32_t pitch = (((a.K + per_word - 1) / per_word) | 1u) * per_word;
-    return launch(distill_thread_kernel<T, GRAD>, (a.n + 255) / 256, 256, 256u * (pitch * (uint32_t)sizeof(T) + (GRAD ? (a.K | 1u) * 4u : 0u)), s, a);
+    const uint32_t lds = 256u * (pitch * (uint32_t)sizeof(T) + (GRAD ? (a.K | 1u) * 4u : 0u));
+    const uint64_t blocks = (a.n + 255) / 256;
+    switch (a.k) {
+      case 1: return launch(distill_thread_kernel<T, 1, GRAD>, blocks, 256, lds, s, a);
+      case 2: return launch(distill_thread_kernel<T, 2, GRAD>, blocks, 256, lds, s, a);
+      case 3: return launch(distill_thread_kernel<T, 3, GRAD>, blocks, 256, lds, s, a);
+      case 4: return launch(distill_thread_kernel<T, 4, GRAD>, blocks, 256, lds, s, a);
+      case 5: return launch(distill_thread_kernel<T, 5, GRAD>, blocks, 256, lds, s, a);
+      default: return launch(distill_thread_kernel<T, 0, GRAD>, blocks, 256, lds, s, a);
+    }
   }
-  if (a.K <= 2048u) return distill_rows<T, 64, GRAD>(a, s);
-  return a.K <= 16384u ? distill_rows<T, 256, GRAD>(a, s) : distill_rows<T, 1024, GRAD>(a, s);
+  const uint32_t packs = (a.K + Pack<T>::N - 1) / Pack<T>::N;
+  if (packs <= 64u) return distill_rows<T, 64, 1, GRAD>(a, s);
+  if (packs <= 128u) return distill_rows<T, 64, 2, GRAD>(a, s);
+  if (packs <= 256u) return distill_rows<T, 64, 4, GRAD>(a, s);
+  if (packs <= 512u) return distill_rows<T, 64, 8, GRAD>(a, s);
+  // few rows: as many threads on each as there are.  Else enough blocks per CU that one row's ends are hidden behind the other rows'
+  // packs -- for the gradient no more than keep their rows in the 256 MB cache until their second read.  (200 M scores, us, 256 / 512 /
+  // 1024 threads: loss of 50257 fp16-sized classes 89 / 109 / 143; gradient 64000 bf16 253 / 249 / 319, 100000 fp32 516 / 454 / 397.)
+  if (a.n <= 512u) return distill_rows<T, 1024, 0, GRAD>(a, s);
+  if (!GRAD) return distill_rows<T, 256, 0, GRAD>(a, s);
+  if (packs <= 1024u) return distill_rows<T, 256, 4, GRAD>(a, s);
+  if (packs <= 2048u) return distill_rows<T, 256, 8, GRAD>(a, s);
+  if (packs <= 4096u) return distill_rows<T, 256, 16, GRAD>(a, s);
+  return packs <= 16384u ? distill_rows<T, 512, 0, GRAD>(a, s) : distill_rows<T, 1024, 0, GRAD>(a, s);
 }
 
 }  // namespace
@@ -1116,8 +1390,11 @@ hipError_t launch_top(const TopArgs& a, uint32_t dtype, bool class_major, hipStr
   if (dtype == DDT_FP32) return top_typed<float>(a, class_major, s);
   return dtype == DDT_FP16 ? top_typed<_Float16>(a, class_major, s) : top_typed<__bf16>(a, class_major, s);
 }
-hipError_t launch_distill(const DistillArgs& a, uint32_t dtype, hipStream_t s) {
-  if (a.n == 0) return hipSuccess;
+hipError_t launch_distill(const DistillArgs& args, uint32_t dtype, hipStream_t s) {
+  if (args.n == 0) return hipSuccess;
+  // student and gradient do not both fit the 256 MB cache: the gradient goes past it (8192 x 128000 bf16 1057 -> 963 us)
+  DistillArgs a = args;
+  a.past_caches = a.n * a.K * (dtype == DDT_FP32 ? 4u : 2u) > (128ull << 20);
   if (dtype == DDT_FP32) return a.grad ? distill_typed<float, true>(a, s) : distill_typed<float, false>(a, s);
   if (dtype == DDT_FP16) return a.grad ? distill_typed<_Float16, true>(a, s) : distill_typed<_Float16, false>(a, s);
   return a.grad ? distill_typed<__bf16, true>(a, s) : distill_typed<__bf16, false>(a, s);

@@ -235,7 +235,8 @@ def top64(x, k, T):
     base = np.where(np.isfinite(m), m, 0)
     with np.errstate(over="ignore", divide="ignore", invalid="ignore"):
         lse = np.log(np.exp((x - base) / T).sum(1)) + base[:, 0] / T
-    return ids, vals, np.where(m[:, 0] == np.inf, np.inf, lse)
+    lse = np.where(m[:, 0] == np.inf, np.inf, lse)
+    return ids, vals, np.where(np.abs(lse) > np.finfo(np.float32).max, np.copysign(np.inf, lse), lse)   # beyond fp32: it rounds to infinity
 
 
 def check_top(engine, x, k, T=1.0):
@@ -312,7 +313,19 @@ def test_top_of_rows_that_tie_or_hold_nothing(engine, kind, K, k, dtype):
         x.copy_(torch.where(c % 2 == 0, 0.0, -0.0)[:, None].expand(K, n))
     elif kind == "one thread":                          # the best stand in the columns that one thread reads
         x.copy_(torch.where((c // 8) % 256 == 5, 9.0 + c / K, -1.0)[:, None].expand(K, n))
-    check_top(engine, x, k)
+    for T in (1.0, 2.0, 0.25):
+        check_top(engine, x, k, T)
+
+
+@pytest.mark.parametrize("K", [10, 300, 5000, 60000])
+def test_sums_of_far_scores(engine, K):
+    """Scores whose multiples leave the range that fp32 counts whole steps in, or fp32 itself: 10^4 to the lowest and largest number."""
+    x = matrix(8, K, "fp32")
+    for r, far in enumerate([1e4, -1e4, 3e6, 1e9, -1e20, 1e37, 3e38, -3e38]):
+        x[:, r] = far + x[:, r] * (1.0 if abs(far) < 1e5 else 0.0)
+        x[K // 2, r] = far
+    check_top(engine, x, 5, 2.0)
+    check_top(engine, x, 5, 0.5)
 
 
 def test_top_rows_at_offsets_past_32_bits(engine):
