@@ -103,6 +103,25 @@ def synth_tuples_host(row0: int, n: int, F: int, dist: int = 0, missing_bits: in
     return out
 
 
+_types = None
+
+
+def _torch_types():
+    """What the class-score calls use of torch, looked up once (torch is imported where it is needed)."""
+    global _types
+    if _types is None:
+        import functools
+        import types
+
+        import torch
+
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
+        _types = types.SimpleNamespace(
+            torch=torch, f32=torch.float32, i32=torch.int32, u32=torch.uint32, i64=torch.int64, raw_stream=raw,
+            codes={torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}, device=functools.lru_cache(None)(lambda i: torch.device("cuda", i)))
+    return _types
+
+
 _distill_cls = None
 
 
@@ -235,43 +254,45 @@ class Engine:
     # ---- class scores: after the trees ---------------------------------------------------------------
     # Matrices are torch tensors [num_classes, n] as classify_device returns them; row-major logits [n, num_classes] go in as
     # logits.t() (a view: the strides say which it is).  Everything is asynchronous on `stream` (default: the device's current
-    # one); results that are not handed in are allocated on it.
-    def _tensor(self, t, what: str, dtype=None, dim=None, shape=None):
-        import torch
-
-        if t.device.type != "cuda" or t.device.index != self.device:
+    # one); results that are not handed in are allocated on it.  The checks are written for the calls that take less time on the
+    # device than in Python: no context, device or dtype object is made on the way through.
+    def _tensor(self, t, what: str, dtype, shape=None) -> int:
+        if not t.is_cuda or t.get_device() != self.device:
             raise ValueError(f"{what}: on {t.device}, the engine is on cuda:{self.device}")
-        if dtype is not None and t.dtype not in (dtype if isinstance(dtype, tuple) else (dtype,)):
+        if t.dtype is not dtype:
             raise ValueError(f"{what}: {t.dtype}, must be {dtype}")
-        if dim is not None and t.dim() != dim:
-            raise ValueError(f"{what}: {t.dim()} dimensions, must be {dim}")
-        if shape is not None and tuple(t.shape) != tuple(shape):
-            raise ValueError(f"{what}: shape {tuple(t.shape)}, must be {tuple(shape)}")
-        return t
-
-    def _packed(self, t, what: str, dtype, shape) -> int:
-        self._tensor(t, what, dtype, shape=shape)
-        if not t.is_contiguous():
-            raise ValueError(f"{what}: must be contiguous")
+        if shape is not None and t.shape != shape:
+            raise ValueError(f"{what}: shape {tuple(t.shape)}, must be {shape}")
         return t.data_ptr()
 
-    def _scores(self, t, what: str) -> _lib.Scores:
-        import torch
+    def _packed(self, t, what: str, dtype, shape) -> int:
+        p = self._tensor(t, what, dtype, shape)
+        if not t.is_contiguous():
+            raise ValueError(f"{what}: must be contiguous")
+        return p
 
-        types = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-        self._tensor(t, what, tuple(types), 2)
-        K, n = t.shape
-        return _lib.Scores(t.data_ptr(), n, t.stride(1), t.stride(0), K, types[t.dtype])
+    def _scores(self, t, what: str, rows: int = 1) -> _lib.Scores:
+        """ddt_scores_t of a tensor whose dimension `rows` counts the rows"""
+        code = _torch_types().codes.get(t.dtype)
+        if code is None:
+            raise ValueError(f"{what}: {t.dtype}, must be one of {list(_torch_types().codes)}")
+        if t.dim() != 2:
+            raise ValueError(f"{what}: {t.dim()} dimensions, must be 2")
+        p, shape, stride = self._tensor(t, what, t.dtype), t.shape, t.stride()
+        return _lib.Scores(p, shape[rows], stride[rows], stride[1 - rows], shape[1 - rows], code)
 
-    def _on(self, stream):
-        """(context that allocates on the stream, its handle)"""
-        import contextlib
+    def _stream(self, stream):
+        """handle of the stream of a call"""
+        return _torch_types().raw_stream(self.device) if stream is None else stream.cuda_stream
 
-        import torch
-
-        if stream is None:
-            return contextlib.nullcontext(), torch.cuda.current_stream(self.device).cuda_stream
-        return torch.cuda.stream(stream), stream.cuda_stream
+    def _empty(self, shape, dtype, stream, strides=None):
+        T = _torch_types()
+        if stream is not None:
+            with T.torch.cuda.stream(stream):
+                return self._empty(shape, dtype, None, strides)
+        if strides is not None:
+            return T.torch.empty_strided(shape, strides, dtype=dtype, device=T.device(self.device))
+        return T.torch.empty(shape, dtype=dtype, device=T.device(self.device))
 
     def adjust_device(self, class_scores, bias=None, allowed=None, history=None, history_first=None, history_prompt=None,
                       repetition=None, frequency=None, presence=None, out=None, stream=None):
@@ -285,48 +306,47 @@ class Engine:
         repetition      fp32 [n]: a class of the history: score / it if positive, else score * it
         frequency       fp32 [n]: minus it for every time the class stands behind the prompt part
         presence        fp32 [n]: minus it if it stands there at all"""
-        import torch
-
+        T = _torch_types()
         s = self._scores(class_scores, "class_scores")
-        K, n = class_scores.shape
-        a, f32, i32 = _lib.Adjust(), torch.float32, torch.int32
+        K, n = s.num_classes, s.rows
+        a = _lib.Adjust()
         if bias is not None:
-            self._tensor(bias, "bias", f32)
-            if tuple(bias.shape) == (K,):
+            a.bias = self._tensor(bias, "bias", T.f32)
+            if bias.shape == (K,):
                 a.bias_class_stride = bias.stride(0)
-            elif tuple(bias.shape) == (K, n):
+            elif bias.shape == (K, n):
                 a.bias_class_stride, a.bias_row_stride = bias.stride()
             else:
                 raise ValueError(f"bias: shape {tuple(bias.shape)}, must be {(K,)} or {(K, n)}")
-            a.bias = bias.data_ptr()
         if allowed is not None:
             words = (K + 31) // 32
-            self._tensor(allowed, "allowed", (i32, torch.uint32))
-            if tuple(allowed.shape) not in ((words,), (n, words)):
+            a.allowed = self._tensor(allowed, "allowed", T.u32 if allowed.dtype is T.u32 else T.i32)
+            if allowed.shape != (words,) and allowed.shape != (n, words):
                 raise ValueError(f"allowed: shape {tuple(allowed.shape)}, must be {(words,)} or {(n, words)}")
             if words > 1 and allowed.stride(-1) != 1:
                 raise ValueError("allowed: the words of a row must be contiguous")
-            a.allowed, a.allowed_row_stride = allowed.data_ptr(), allowed.stride(0) if allowed.dim() == 2 and n > 1 else 0
+            a.allowed_row_stride = allowed.stride(0) if n > 1 and allowed.dim() == 2 else 0
         if history is not None:
             if history_first is None:
                 raise ValueError("history without history_first")
-            a.history = self._packed(history, "history", i32, (history.numel(),))
             a.history_len = history.numel()
-            a.history_first = self._packed(history_first, "history_first", torch.int64, (n + 1,))
+            a.history = self._packed(history, "history", T.i32, (a.history_len,))
+            a.history_first = self._packed(history_first, "history_first", T.i64, (n + 1,))
             if history_prompt is not None:
-                a.history_prompt = self._packed(history_prompt, "history_prompt", i32, (n,))
-            for name, t in (("repetition", repetition), ("frequency", frequency), ("presence", presence)):
-                if t is not None:
-                    setattr(a, name, self._packed(t, name, f32, (n,)))
-        elif any(t is not None for t in (history_first, history_prompt, repetition, frequency, presence)):
+                a.history_prompt = self._packed(history_prompt, "history_prompt", T.i32, (n,))
+            if repetition is not None:
+                a.repetition = self._packed(repetition, "repetition", T.f32, (n,))
+            if frequency is not None:
+                a.frequency = self._packed(frequency, "frequency", T.f32, (n,))
+            if presence is not None:
+                a.presence = self._packed(presence, "presence", T.f32, (n,))
+        elif not (history_first is None and history_prompt is None and repetition is None and frequency is None and presence is None):
             raise ValueError("history_first, history_prompt and penalties need a history")
-        on, handle = self._on(stream)
-        with on:
-            if out is None:
-                out = torch.empty_strided((K, n), (1, K) if s.class_stride == 1 and (s.row_stride >= K or n <= 1) else (n, 1),
-                                          dtype=class_scores.dtype, device=class_scores.device)
-            o = self._scores(out, "out")
-            self._check(self._L.ddt_adjust_scores_device(self._h, C.byref(s), C.byref(a), C.byref(o), handle))
+        if out is None:
+            row_major = s.class_stride == 1 and (s.row_stride >= K or n <= 1)
+            out = self._empty((K, n), class_scores.dtype, stream, (1, K) if row_major else (n, 1))
+        o = self._scores(out, "out")
+        self._check(self._L.ddt_adjust_scores_device(self._h, C.byref(s), C.byref(a), C.byref(o), self._stream(stream)))
         return out
 
     def top_device(self, class_scores, k: int, temperature: float = 1.0, ids=None, values=None, lse=None, stream=None):
@@ -334,18 +354,15 @@ class Engine:
         (ids int32 [n, k], values fp32 [n, k], lse fp32 [n] = log sum exp(score / temperature) over all classes): the class's
         probability is exp(values / temperature - lse).  Rows with fewer candidates (NaN and -inf are none) end in id -1, value
         -inf.  (ddt_top_scores_device)"""
-        import torch
-
+        T = _torch_types()
         s = self._scores(class_scores, "class_scores")
-        n, dev = class_scores.shape[1], class_scores.device
-        on, handle = self._on(stream)
-        with on:
-            ids = torch.empty((n, k), dtype=torch.int32, device=dev) if ids is None else ids
-            values = torch.empty((n, k), dtype=torch.float32, device=dev) if values is None else values
-            lse = torch.empty(n, dtype=torch.float32, device=dev) if lse is None else lse
-            self._check(self._L.ddt_top_scores_device(
-                self._h, C.byref(s), k, temperature, self._packed(ids, "ids", torch.int32, (n, k)),
-                self._packed(values, "values", torch.float32, (n, k)), self._packed(lse, "lse", torch.float32, (n,)), handle))
+        n = s.rows
+        ids = self._empty((n, k), T.i32, stream) if ids is None else ids
+        values = self._empty((n, k), T.f32, stream) if values is None else values
+        lse = self._empty((n,), T.f32, stream) if lse is None else lse
+        self._check(self._L.ddt_top_scores_device(
+            self._h, C.byref(s), k, temperature, self._packed(ids, "ids", T.i32, (n, k)),
+            self._packed(values, "values", T.f32, (n, k)), self._packed(lse, "lse", T.f32, (n,)), self._stream(stream)))
         return ids, values, lse
 
     def top_classes_device(self, d_tuples, k: int, temperature: float = 1.0, stream=None, **adjust):
@@ -362,32 +379,25 @@ class Engine:
                 self.adjust_device(scores, out=scores, **adjust)
             return self.top_device(scores, k, temperature)
 
-    def _teacher(self, student, ids, values, lse, temperature) -> _lib.Teacher:
-        import torch
-
-        n, k = student.shape[0], ids.shape[-1]
-        self._tensor(ids, "ids", torch.int32, shape=(n, k))
-        self._tensor(values, "values", torch.float32, shape=(n, k))
-        if (k > 1 and (ids.stride(1) != 1 or values.stride(1) != 1)) or (n > 1 and ids.stride(0) != values.stride(0)):
+    def _teacher(self, n, ids, values, lse, temperature) -> _lib.Teacher:
+        T = _torch_types()
+        k = ids.shape[-1] if ids.dim() else 0
+        p, v = self._tensor(ids, "ids", T.i32, (n, k)), self._tensor(values, "values", T.f32, (n, k))
+        by_row, by_entry = ids.stride()
+        if ids.stride() != values.stride() and n > 1 or k > 1 and (by_entry != 1 or values.stride(1) != 1):
             raise ValueError("ids, values: rows must be contiguous and stand equally far apart")
-        t = _lib.Teacher(ids.data_ptr(), values.data_ptr(), ids.stride(0) if n > 1 else k, None, k, temperature)
-        if lse is not None:
-            t.lse = self._packed(lse, "lse", torch.float32, (n,))
-        return t
+        return _lib.Teacher(p, v, by_row if n > 1 else k, None if lse is None else self._packed(lse, "lse", T.f32, (n,)), k, temperature)
 
     def distill_device(self, student, ids, values, lse=None, temperature: float = 1.0, loss=None, stream=None):
         """KL divergence of a student's softmax (scores [n, K], row-major) from a teacher's top scores (ids, values, lse of
         top_device at the same temperature) -> loss fp32 [n].  lse None: the teacher's probabilities are normalised over the
         listed classes; otherwise everything it does not list is one more outcome.  (ddt_distill_device)"""
-        import torch
-
-        s = self._scores(student.t() if student.dim() == 2 else student, "student")
-        t = self._teacher(student, ids, values, lse, temperature)
-        on, handle = self._on(stream)
-        with on:
-            loss = torch.empty(student.shape[0], dtype=torch.float32, device=student.device) if loss is None else loss
-            self._check(self._L.ddt_distill_device(self._h, C.byref(s), C.byref(t),
-                                                   self._packed(loss, "loss", torch.float32, (student.shape[0],)), handle))
+        T = _torch_types()
+        s = self._scores(student, "student", rows=0)
+        t = self._teacher(s.rows, ids, values, lse, temperature)
+        loss = self._empty((s.rows,), T.f32, stream) if loss is None else loss
+        self._check(self._L.ddt_distill_device(self._h, C.byref(s), C.byref(t), self._packed(loss, "loss", T.f32, (s.rows,)),
+                                               self._stream(stream)))
         return loss
 
     def distill_grad_device(self, student, ids, values, lse=None, row_weight=None, temperature: float = 1.0, loss=None, grad=None,
@@ -395,22 +405,18 @@ class Engine:
         """distill_device and, from the same pass over the student's scores, the gradient of sum(row_weight * loss) by them ->
         (loss fp32 [n], grad [n, K] of the student's type); row_weight fp32 [n] (any stride; None = 1), `grad` may be `student`.
         (ddt_distill_grad_device)"""
-        import torch
-
-        s = self._scores(student.t() if student.dim() == 2 else student, "student")
-        t = self._teacher(student, ids, values, lse, temperature)
-        n = student.shape[0]
+        T = _torch_types()
+        s = self._scores(student, "student", rows=0)
+        n = s.rows
+        t = self._teacher(n, ids, values, lse, temperature)
+        w, w_stride = None, 0
         if row_weight is not None:
-            self._tensor(row_weight, "row_weight", torch.float32, shape=(n,))
-        on, handle = self._on(stream)
-        with on:
-            loss = torch.empty(n, dtype=torch.float32, device=student.device) if loss is None else loss
-            grad = torch.empty(student.shape, dtype=student.dtype, device=student.device) if grad is None else grad
-            g = self._scores(grad.t(), "grad")
-            self._check(self._L.ddt_distill_grad_device(
-                self._h, C.byref(s), C.byref(t), row_weight.data_ptr() if row_weight is not None else None,
-                row_weight.stride(0) if row_weight is not None and n > 1 else 0,
-                self._packed(loss, "loss", torch.float32, (n,)), C.byref(g), handle))
+            w, w_stride = self._tensor(row_weight, "row_weight", T.f32, (n,)), row_weight.stride(0) if n > 1 else 0
+        loss = self._empty((n,), T.f32, stream) if loss is None else loss
+        grad = self._empty((n, s.num_classes), student.dtype, stream) if grad is None else grad
+        g = self._scores(grad, "grad", rows=0)
+        self._check(self._L.ddt_distill_grad_device(self._h, C.byref(s), C.byref(t), w, w_stride,
+                                                    self._packed(loss, "loss", T.f32, (n,)), C.byref(g), self._stream(stream)))
         return loss, grad
 
     def distill(self, student, ids, values, lse=None, temperature: float = 1.0):
