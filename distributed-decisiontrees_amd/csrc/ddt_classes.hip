@@ -40,6 +40,18 @@ __device__ __forceinline__ void load_pack(const T* row, uint32_t c, uint32_t end
     for (uint32_t i = 0; i < N; ++i) x[i] = c + i < end ? (float)row[c + i] : fill;
   }
 }
+// four packs, STEP packs apart, some of them partial or behind the end: `fill` there
+template <class T, uint32_t STEP>
+__device__ __forceinline__ void load_last_packs(const T* row, uint32_t p, uint32_t end, float fill, float (&x)[4 * Pack<T>::N]) {
+  constexpr uint32_t N = Pack<T>::N;
+#pragma unroll
+  for (uint32_t u = 0; u < 4; ++u) {
+    float v[N];
+    load_pack(row, (p + u * STEP) * N, end, fill, v);
+#pragma unroll
+    for (uint32_t i = 0; i < N; ++i) x[u * N + i] = v[i];
+  }
+}
 // four whole packs, STEP packs apart
 template <class T, uint32_t STEP>
 __device__ __forceinline__ void load_packs(const T* row, uint32_t p, float (&x)[4 * Pack<T>::N]) {
@@ -412,7 +424,7 @@ struct RunSum {
     return fminf(fmaxf(fmaf(fabsf(m * c), 0x1p-23f, m * c), -FLT_MAX), FLT_MAX);
   }
   template <uint32_t M>
-  __device__ __forceinline__ void add(const float (&x)[M], float c) {
+  __device__ __forceinline__ float add(const float (&x)[M], float c) {  // -> the largest of x
     float pm = x[0];
 #pragma unroll
     for (uint32_t i = 1; i < M; ++i) pm = fmaxf(pm, x[i]);
@@ -425,6 +437,7 @@ struct RunSum {
 #pragma unroll
     for (uint32_t i = 0; i < M; ++i) t[i & 3u] += exp2_fast(fmaf(x[i], c, -r));
     s += (t[0] + t[1]) + (t[2] + t[3]);
+    return pm;
   }
   // over the wave; plain(M) = this lane's sum of exp2((x - M) c)
   template <class Plain>
@@ -556,21 +569,31 @@ __global__ __launch_bounds__(256) void top_thread_kernel(const TopArgs a) {
   }
 }
 
-// the kk-th largest of the keys in a wave's registers (E per lane): greedy from the top bit, counted with ballots
+// A number that at least kk of the keys in a wave's registers (E per lane) reach: greedy from the top bit, counted with ballots.  Bits
+// below the 16th (sign, exponent and 7 bits of a score) are looked at only while more than kk + slack keys reach it: slack 0 and keys that
+// tie across kk give the kk-th largest key itself.  Fewer keys than kk: 0.
 template <int E>
-__device__ __forceinline__ uint32_t wave_kth_key(const uint32_t (&key)[E], uint32_t kk, uint32_t low) {
-  uint32_t t = 0u;
+__device__ __forceinline__ uint32_t wave_kth_key(const uint32_t (&key)[E], uint32_t kk, uint32_t slack, uint32_t low) {
+  uint32_t t = 0u, reach = 64u * E;
   for (int bit = 31; bit >= (int)low; --bit) {
+    if (bit < 16 && reach <= kk + slack) break;
     const uint32_t cand = t | (1u << bit);
     uint32_t cnt = 0u;
 #pragma unroll
     for (int i = 0; i < E; ++i) cnt += __popcll(__ballot(key[i] >= cand));
     if (cnt >= kk) {
-      t = cand;
-      if (cnt == kk) break;  // exactly the kk best: a lower bound that admits no others
+      t = cand, reach = cnt;
+      if (cnt == kk) break;
     }
   }
   return t;
+}
+// how many of `count` candidates in LDS are better than `mine`
+__device__ __forceinline__ uint32_t rank_of(uint64_t mine, const uint64_t* list, uint32_t count) {
+  uint32_t rank = 0u;
+#pragma unroll 8
+  for (uint32_t j = 0; j < count; ++j) rank += list[j] > mine;
+  return rank;
 }
 
 // up to 2048 classes: a wave per row, all its keys in registers (P packs per lane).  Class-major rows are staged through LDS, 16 at a
@@ -621,12 +644,12 @@ __global__ __launch_bounds__(top_wave_waves(CM) * 64) void top_wave_kernel(const
       for (int i = 0; i < E; ++i) e.s += exp2_fast((x[i] - e.m) * c2);
       e.s = wave_sum(e.s);
       if (a.lse && lane == 0u) a.lse[row] = log_sum(e, 1.0 / a.temperature);
-      // A bound that at least k scores reach: the k-th largest of the lanes' best, to 16 bits (sign, exponent, 7 bits: no more than a
-      // few scores stand between the exact one and this).  What reaches it is listed and ranked.
+      // A bound that at least k scores reach: the k-th largest of the lanes' best, or a little below it.  What reaches it is listed and
+      // ranked.
       uint32_t count = kWaveList + 1u;
       if (a.k <= 64u) {
         const uint32_t lane_key[1] = {score_key(best)};
-        const uint32_t t = wave_kth_key(lane_key, a.k, 16u);
+        const uint32_t t = wave_kth_key(lane_key, a.k, a.k, low_bits<T>());
         const float bound = t ? key_score(t) : -FLT_MAX;
         count = 0u;
 #pragma unroll
@@ -644,7 +667,7 @@ __global__ __launch_bounds__(top_wave_waves(CM) * 64) void top_wave_kernel(const
 #pragma unroll
         for (int i = 0; i < E; ++i) key[i] = score_key(x[i]), valid += __popcll(__ballot(key[i] != 0u));
         const uint32_t kk = valid < a.k ? valid : a.k;
-        uint32_t t = wave_kth_key(key, kk, low_bits<T>());
+        uint32_t t = wave_kth_key(key, kk, 0u, low_bits<T>());
         if (t == 0u) t = 1u;  // (fewer than k candidates: all of them)
         // everything from t up, if that is kk; else what lies above t's score, and of the classes with t's score the lowest ones
         uint32_t ge = 0u, gt = 0u;
@@ -683,8 +706,7 @@ __global__ __launch_bounds__(top_wave_waves(CM) * 64) void top_wave_kernel(const
           continue;
         }
         const uint64_t mine = list[i];
-        uint32_t rank = 0u;
-        for (uint32_t j = 0; j < count; ++j) rank += list[j] > mine;
+        const uint32_t rank = rank_of(mine, list, count);
         if (rank < a.k) write_candidate(a, row, rank, mine);
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -693,34 +715,62 @@ __global__ __launch_bounds__(top_wave_waves(CM) * 64) void top_wave_kernel(const
   }
 }
 
-// many classes: a block of NT threads per row.  One pass keeps each thread's largest score and its sum of exponentials; the k-th largest
-// of the NT maxima is a bound that at least k scores reach, and only the threads whose maximum reaches it -- about k of them -- read
-// their scores a second time to list the candidates.  Rows with more candidates than the list holds (scores that tie, or stand in few
-// threads) are narrowed down by counting, bit by bit, over the threads that reach the bound.
-constexpr uint32_t kListCap = 1024;
+// many classes: a block of NT threads per row, four packs of a thread at a time (a chunk).  One pass keeps the sum of exponentials, the
+// thread's largest score, and the largest score of each group of chunks (at most 16 groups; to 16 bits, in LDS).  The k-th largest of the
+// threads' maxima is a bound that at least k scores reach, and only the groups that reach it -- about k of them, 64 packs of
+// 128000 -- are read a second time to list the candidates.  Rows with more candidates than the list holds (scores that tie, or stand
+// in few threads) are narrowed down by counting, bit by bit, over the threads that reach the bound.
+// 512 x 128000 bf16, k = 64: 25 us for the pass (5.2 TB/s), 3 for the bound, 3 for the second look, 2 for the ranks.
+constexpr uint32_t kListCap = 1024, kGroups = 16;
+constexpr uint32_t top_block_words(uint32_t threads) {  // LDS
+  return 2u * kListCap + threads + 2u * (threads / 64u) + 4u + threads / 64u + kGroups * threads / 2u;
+}
+__device__ __forceinline__ uint32_t quad_max(uint32_t v) {
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true));
+  return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true));
+}
 template <class T, int NT>
 __global__ __launch_bounds__(NT) void top_block_kernel(const TopArgs a) {
   constexpr uint32_t N = Pack<T>::N, kWaves = NT / 64;
   uint64_t* list = reinterpret_cast<uint64_t*>(lds_words);         // [kListCap]
   uint32_t* maxima = lds_words + 2 * kListCap;                     // [NT]
   float* part = reinterpret_cast<float*>(maxima + NT);             // [2 * kWaves]
-  uint32_t* ctl = reinterpret_cast<uint32_t*>(part + 2 * kWaves);  // [0] bound, [1] candidates, [2] threads that hold them, [3 ..] counts per wave
+  uint32_t* ctl = reinterpret_cast<uint32_t*>(part + 2 * kWaves);  // [0] bound, [1] candidates, [2] groups that hold them, [4 ..] counts per wave
+  uint16_t* group_max = reinterpret_cast<uint16_t*>(ctl + 4 + kWaves);  // [kGroups][NT]
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
-  const uint32_t packs = (a.K + N - 1u) / N;
+  const uint32_t packs = (a.K + N - 1u) / N, chunks = (packs + 4u * NT - 1u) / (4u * NT);
+  const uint32_t per_group = (chunks + kGroups - 1u) / kGroups;  // chunks
   const float c2 = (float)(kLog2e / a.temperature);
   for (uint64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
     const T* in = static_cast<const T*>(a.in) + row * a.stride;
     RunSum run(c2);
-    uint32_t p0 = 0;
-    for (; (p0 + 4u * NT) * N <= a.K; p0 += 4u * NT) {  // four packs of a thread in flight
+    float largest = -kInf;  // of the group
+    uint32_t p0 = 0, groups = 0, left = per_group;
+    __syncthreads();  // the row before is written
+    auto chunk_done = [&](float pm) {
+      largest = fmaxf(largest, pm);
+      if (--left == 0u) {
+        group_max[groups * NT + tid] = (uint16_t)(score_key(largest) >> 16);
+        ++groups, left = per_group, largest = -kInf;
+      }
+    };
+    for (; (p0 + 4u * NT) * N <= a.K; p0 += 4u * NT) {
       float x[4 * N];
       load_packs<T, NT>(in, p0 + tid, x);
-      run.add(x, c2);
+      chunk_done(run.add(x, c2));
     }
-    for (uint32_t p = p0 + tid; p < packs; p += NT) {
-      float x[N];
-      load_pack(in, p * N, a.K, -kInf, x);
-      run.add(x, c2);
+    if (p0 < packs) {
+      float pm = -kInf;
+      if (p0 + tid < packs) {
+        float x[4 * N];
+        load_last_packs<T, NT>(in, p0 + tid, a.K, -kInf, x);
+        pm = run.add(x, c2);
+      }
+      left = 1u;
+      chunk_done(pm);
+    } else if (left != per_group) {
+      left = 1u;
+      chunk_done(-kInf);
     }
     const uint32_t best = score_key(run.m);  // (a thread without a candidate counts with the lowest score: the bound only sinks)
     const ExpSum e = run.finish(c2, [&](float M) {
@@ -733,17 +783,29 @@ __global__ __launch_bounds__(NT) void top_block_kernel(const TopArgs a) {
       }
       return t;
     });
-    __syncthreads();  // the row before is written
-    maxima[tid] = best;
+    const bool quads = a.k <= NT / 8u;  // few wanted: the largest of four lanes will do, and is a quarter to search
+    if (quads) {
+      const uint32_t q = quad_max(best);
+      if ((tid & 3u) == 0u) maxima[tid >> 2] = q;
+    } else {
+      maxima[tid] = best;
+    }
     if (lane == 0u) part[2 * wave] = e.m, part[2 * wave + 1] = e.s;
     if (tid == 0u) ctl[1] = 0u, ctl[2] = 0u;
     __syncthreads();
     if (wave == 0u) {
-      constexpr int E = NT / 64;
-      uint32_t key[E];
+      uint32_t t;
+      if (quads) {
+        uint32_t key[NT / 256];
 #pragma unroll
-      for (int i = 0; i < E; ++i) key[i] = maxima[i * 64 + lane];
-      const uint32_t t = wave_kth_key(key, a.k, low_bits<T>());
+        for (int i = 0; i < NT / 256; ++i) key[i] = maxima[i * 64 + lane];
+        t = wave_kth_key(key, a.k, a.k / 4u, low_bits<T>());
+      } else {
+        uint32_t key[NT / 64];
+#pragma unroll
+        for (int i = 0; i < NT / 64; ++i) key[i] = maxima[i * 64 + lane];
+        t = wave_kth_key(key, a.k, a.k / 4u, low_bits<T>());
+      }
       if (lane == 0u) ctl[0] = t ? t : 1u;
     } else if (wave == 1u && a.lse) {
       ExpSum w;
@@ -754,31 +816,39 @@ __global__ __launch_bounds__(NT) void top_block_kernel(const TopArgs a) {
     __syncthreads();
     const uint32_t bound = ctl[0];
     const bool mine = best >= bound;
-    uint32_t* owners = maxima;  // threads whose packs hold candidates
-    if (mine) owners[atomicAdd(&ctl[2], 1u)] = tid;
-    __syncthreads();
-    {
-      // their packs, dealt out over the whole block: item i = pack (i mod per) of owner (i div per)
-      const uint32_t per = (packs + NT - 1u) / NT, items = ctl[2] * per, magic = 0xFFFFFFFFu / per + 1u;  // (i per < 2^32; per = 1: magic 0)
-      for (uint32_t i0 = tid; i0 < items; i0 += 4u * NT) {
-        float x[4][N];
-        uint32_t c[4];
-#pragma unroll
-        for (uint32_t u = 0; u < 4; ++u) {
-          const uint32_t i = i0 + u * NT, o = per == 1u ? i : __umulhi(i, magic);
-          c[u] = i < items ? (owners[o] + (i - o * per) * NT) * N : a.K;
-          load_pack(in, c[u], a.K, -kInf, x[u]);
+    uint32_t* owners = maxima;  // group * NT + thread, of the groups that hold candidates
+    if (mine)
+      for (uint32_t g = 0; g < groups; ++g)
+        if (group_max[g * NT + tid] >= bound >> 16) {
+          const uint32_t slot = atomicAdd(&ctl[2], 1u);
+          if (slot < NT) owners[slot] = g * NT + tid;
         }
+    __syncthreads();
+    auto look = [&](const float (&x)[N], uint32_t c) {
 #pragma unroll
-        for (uint32_t u = 0; u < 4; ++u)
-#pragma unroll
-          for (uint32_t j = 0; j < N; ++j) {
-            const uint32_t key = score_key(x[u][j]);
-            if (key >= bound) {
-              const uint32_t slot = atomicAdd(&ctl[1], 1u);
-              if (slot < kListCap) list[slot] = candidate(key, c[u] + j);
-            }
-          }
+      for (uint32_t j = 0; j < N; ++j) {
+        const uint32_t key = score_key(x[j]);
+        if (key >= bound) {
+          const uint32_t slot = atomicAdd(&ctl[1], 1u);
+          if (slot < kListCap) list[slot] = candidate(key, c + j);
+        }
+      }
+    };
+    if (ctl[2] <= NT) {
+      // their packs, dealt out over the whole block: item i = pack (i mod per) of owner (i div per)
+      const uint32_t per = 4u * per_group, items = ctl[2] * per, magic = 0xFFFFFFFFu / per + 1u;  // (i per < 2^32, per >= 4)
+      for (uint32_t i = tid; i < items; i += NT) {
+        const uint32_t o = __umulhi(i, magic), own = owners[o], g = own / NT;
+        const uint32_t c = ((g * per + i - o * per) * NT + own % NT) * N;
+        float x[N];
+        load_pack(in, c, a.K, -kInf, x);
+        look(x, c);
+      }
+    } else if (mine) {
+      for (uint32_t p = tid; p < packs; p += NT) {
+        float x[N];
+        load_pack(in, p * N, a.K, -kInf, x);
+        look(x, p * N);
       }
     }
     __syncthreads();
@@ -801,10 +871,10 @@ __global__ __launch_bounds__(NT) void top_block_kernel(const TopArgs a) {
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) n += __shfl_xor(n, d);
         __syncthreads();
-        if (lane == 0u) ctl[3 + wave] = n;
+        if (lane == 0u) ctl[4 + wave] = n;
         __syncthreads();
         uint32_t sum = 0u;
-        for (uint32_t w = 0; w < kWaves; ++w) sum += ctl[3 + w];
+        for (uint32_t w = 0; w < kWaves; ++w) sum += ctl[4 + w];
         return sum;
       };
       uint32_t t = bound;  // raised to the kk-th largest key: bits below the bound's differing ones are tried from the top
@@ -845,8 +915,7 @@ __global__ __launch_bounds__(NT) void top_block_kernel(const TopArgs a) {
         continue;
       }
       const uint64_t v = list[i];
-      uint32_t rank = 0u;
-      for (uint32_t j = 0; j < count; ++j) rank += list[j] > v;
+      const uint32_t rank = rank_of(v, list, count);
       if (rank < a.k) write_candidate(a, row, rank, v);
     }
   }
@@ -1358,7 +1427,7 @@ hipError_t top_wave(const TopArgs& a, hipStream_t s) {
 }
 template <class T, int NT>
 hipError_t top_block(const TopArgs& a, hipStream_t s) {
-  return launch(top_block_kernel<T, NT>, a.n, NT, 8u * kListCap + 4u * NT + 8u * (NT / 64) + 4u * (3u + NT / 64), s, a);
+  return launch(top_block_kernel<T, NT>, a.n, NT, 4u * top_block_words(NT), s, a);
 }
 template <class T>
 hipError_t top_typed(const TopArgs& a, bool class_major, hipStream_t s) {

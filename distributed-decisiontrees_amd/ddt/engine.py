@@ -110,7 +110,6 @@ def _torch_types():
     """What the class-score calls use of torch, looked up once (torch is imported where it is needed)."""
     global _types
     if _types is None:
-        import functools
         import types
 
         import torch
@@ -118,7 +117,7 @@ def _torch_types():
         raw = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
         _types = types.SimpleNamespace(
             torch=torch, f32=torch.float32, i32=torch.int32, u32=torch.uint32, i64=torch.int64, raw_stream=raw,
-            codes={torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}, device=functools.lru_cache(None)(lambda i: torch.device("cuda", i)))
+            codes={torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
     return _types
 
 
@@ -285,14 +284,13 @@ class Engine:
         """handle of the stream of a call"""
         return _torch_types().raw_stream(self.device) if stream is None else stream.cuda_stream
 
-    def _empty(self, shape, dtype, stream, strides=None):
-        T = _torch_types()
+    @staticmethod
+    def _empty(like, shape, dtype, stream, strides=None):
+        """uninitialised tensor on the device of `like`, allocated on the stream of the call"""
         if stream is not None:
-            with T.torch.cuda.stream(stream):
-                return self._empty(shape, dtype, None, strides)
-        if strides is not None:
-            return T.torch.empty_strided(shape, strides, dtype=dtype, device=T.device(self.device))
-        return T.torch.empty(shape, dtype=dtype, device=T.device(self.device))
+            with _torch_types().torch.cuda.stream(stream):
+                return Engine._empty(like, shape, dtype, None, strides)
+        return like.new_empty(shape, dtype=dtype) if strides is None else like.new_empty_strided(shape, strides)
 
     def adjust_device(self, class_scores, bias=None, allowed=None, history=None, history_first=None, history_prompt=None,
                       repetition=None, frequency=None, presence=None, out=None, stream=None):
@@ -344,7 +342,7 @@ class Engine:
             raise ValueError("history_first, history_prompt and penalties need a history")
         if out is None:
             row_major = s.class_stride == 1 and (s.row_stride >= K or n <= 1)
-            out = self._empty((K, n), class_scores.dtype, stream, (1, K) if row_major else (n, 1))
+            out = self._empty(class_scores, (K, n), None, stream, (1, K) if row_major else (n, 1))
         o = self._scores(out, "out")
         self._check(self._L.ddt_adjust_scores_device(self._h, C.byref(s), C.byref(a), C.byref(o), self._stream(stream)))
         return out
@@ -357,9 +355,9 @@ class Engine:
         T = _torch_types()
         s = self._scores(class_scores, "class_scores")
         n = s.rows
-        ids = self._empty((n, k), T.i32, stream) if ids is None else ids
-        values = self._empty((n, k), T.f32, stream) if values is None else values
-        lse = self._empty((n,), T.f32, stream) if lse is None else lse
+        ids = self._empty(class_scores, (n, k), T.i32, stream) if ids is None else ids
+        values = self._empty(class_scores, (n, k), T.f32, stream) if values is None else values
+        lse = self._empty(class_scores, (n,), T.f32, stream) if lse is None else lse
         self._check(self._L.ddt_top_scores_device(
             self._h, C.byref(s), k, temperature, self._packed(ids, "ids", T.i32, (n, k)),
             self._packed(values, "values", T.f32, (n, k)), self._packed(lse, "lse", T.f32, (n,)), self._stream(stream)))
@@ -395,7 +393,7 @@ class Engine:
         T = _torch_types()
         s = self._scores(student, "student", rows=0)
         t = self._teacher(s.rows, ids, values, lse, temperature)
-        loss = self._empty((s.rows,), T.f32, stream) if loss is None else loss
+        loss = self._empty(student, (s.rows,), T.f32, stream) if loss is None else loss
         self._check(self._L.ddt_distill_device(self._h, C.byref(s), C.byref(t), self._packed(loss, "loss", T.f32, (s.rows,)),
                                                self._stream(stream)))
         return loss
@@ -412,8 +410,8 @@ class Engine:
         w, w_stride = None, 0
         if row_weight is not None:
             w, w_stride = self._tensor(row_weight, "row_weight", T.f32, (n,)), row_weight.stride(0) if n > 1 else 0
-        loss = self._empty((n,), T.f32, stream) if loss is None else loss
-        grad = self._empty((n, s.num_classes), student.dtype, stream) if grad is None else grad
+        loss = self._empty(student, (n,), T.f32, stream) if loss is None else loss
+        grad = self._empty(student, (n, s.num_classes), student.dtype, stream) if grad is None else grad
         g = self._scores(grad, "grad", rows=0)
         self._check(self._L.ddt_distill_grad_device(self._h, C.byref(s), C.byref(t), w, w_stride,
                                                     self._packed(loss, "loss", T.f32, (n,)), C.byref(g), self._stream(stream)))
