@@ -114,7 +114,13 @@ struct HeldPack {
   __device__ __forceinline__ void hold() { asm volatile("" : "+v"(w[0]), "+v"(w[1]), "+v"(w[2]), "+v"(w[3])); }
 };
 
+// What is computed from a thread's number is the same for every row, and the compiler keeps all of it across the loop over rows: twice the
+// registers for nothing (most blocks take one row).  forget() makes the number new to it.
 __device__ __forceinline__ void forget(uint32_t& v) { asm volatile("" : "+v"(v)); }
+__device__ __forceinline__ uint32_t forgotten(uint32_t v) {
+  forget(v);
+  return v;
+}
 
 // x ^ 2: the hardware instruction (1 ulp; results below 2^-126 may come back as 0 -- nothing next to a sum whose largest term is 1)
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -274,13 +280,14 @@ __global__ __launch_bounds__(NT) void adjust_rows_kernel(const AdjustArgs a, con
     const uint32_t c0 = (uint32_t)(tile - rt * t.class_tiles) * t.classes;
     const uint32_t rows = (uint32_t)(a.n - r0 < t.rows ? a.n - r0 : t.rows);
     const uint32_t C = a.K - c0 < t.classes ? a.K - c0 : t.classes;
+    const uint32_t tid = forgotten(threadIdx.x);
     HeldPack<T> raw[ITER];
     float bias[ITER][N];
     uint32_t bits[ITER], q[ITER], cl[ITER];
     RowPenalty pen[ITER];
 #pragma unroll
     for (int u = 0; u < ITER; ++u) {
-      const uint32_t idx = threadIdx.x + (uint32_t)u * NT;
+      const uint32_t idx = tid + (uint32_t)u * NT;
       q[u] = t.rows == 1u ? 0u : ppr == 1u ? idx : __umulhi(idx, t.magic), cl[u] = (idx - q[u] * ppr) * N;
       const uint32_t c = c0 + cl[u];
       const uint64_t r = r0 + q[u];
@@ -530,8 +537,9 @@ __global__ __launch_bounds__(256) void top_thread_kernel(const TopArgs a) {
       stage_rows(in, r0, rows, a.K, a.stride, stage, pitch);
       __syncthreads();
     }
-    if (threadIdx.x >= rows) continue;
-    const uint64_t row = r0 + threadIdx.x;
+    const uint32_t tid = forgotten(threadIdx.x);
+    if (tid >= rows) continue;
+    const uint64_t row = r0 + tid;
     float v[KK];
     int32_t id[KK];
 #pragma unroll
@@ -542,7 +550,7 @@ __global__ __launch_bounds__(256) void top_thread_kernel(const TopArgs a) {
       T next[kAhead];
 #pragma unroll
       for (uint32_t i = 0; i < kAhead; ++i)
-        if (c0 + i < a.K) next[i] = CM ? in[(c0 + i) * a.stride + row] : stage[threadIdx.x * pitch + c0 + i];
+        if (c0 + i < a.K) next[i] = CM ? in[(c0 + i) * a.stride + row] : stage[tid * pitch + c0 + i];
 #pragma unroll
       for (uint32_t i = 0; i < kAhead; ++i) {
         if (c0 + i >= a.K) break;
@@ -609,7 +617,7 @@ template <class T, bool CM, int P>
 __global__ __launch_bounds__(top_wave_waves(CM) * 64) void top_wave_kernel(const TopArgs a) {
   constexpr int N = (int)Pack<T>::N, E = P * N;
   constexpr uint32_t kRows = top_wave_rows(CM), kWaves = top_wave_waves(CM);
-  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+  const uint32_t wave = threadIdx.x >> 6;
   uint64_t* list = reinterpret_cast<uint64_t*>(lds_words) + wave * wave_list(a.k);  // the wave's selected candidates
   T* stage = reinterpret_cast<T*>(reinterpret_cast<uint64_t*>(lds_words) + kWaves * wave_list(a.k));  // class-major: [K][16] scores
   const float c2 = (float)(kLog2e / a.temperature);
@@ -623,6 +631,7 @@ __global__ __launch_bounds__(top_wave_waves(CM) * 64) void top_wave_kernel(const
     }
     for (uint32_t rr = wave; rr < kRows && r0 + rr < a.n; rr += kWaves) {
       const uint64_t row = r0 + rr;
+      const uint32_t lane = forgotten(threadIdx.x & 63u);
       float x[E];
       float best = -kInf;
 #pragma unroll
@@ -737,12 +746,12 @@ __global__ __launch_bounds__(NT) void top_block_kernel(const TopArgs a) {
   float* part = reinterpret_cast<float*>(maxima + NT);             // [2 * kWaves]
   uint32_t* ctl = reinterpret_cast<uint32_t*>(part + 2 * kWaves);  // [0] bound, [1] candidates, [2] groups that hold them, [4 ..] counts per wave
   uint16_t* group_max = reinterpret_cast<uint16_t*>(ctl + 4 + kWaves);  // [kGroups][NT]
-  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
   const uint32_t packs = (a.K + N - 1u) / N, chunks = (packs + 4u * NT - 1u) / (4u * NT);
   const uint32_t per_group = (chunks + kGroups - 1u) / kGroups;  // chunks
   const float c2 = (float)(kLog2e / a.temperature);
   for (uint64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
     const T* in = static_cast<const T*>(a.in) + row * a.stride;
+    const uint32_t tid = forgotten(threadIdx.x), lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     RunSum run(c2);
     float largest = -kInf;  // of the group
     uint32_t p0 = 0, groups = 0, left = per_group;
@@ -1013,7 +1022,7 @@ __host__ __device__ constexpr uint32_t distill_words(uint32_t K, uint32_t k, uin
 template <class T, int NT, int P, bool GRAD>
 __global__ __launch_bounds__(NT == 64 ? 256 : NT) void distill_kernel(const DistillArgs a) {
   constexpr uint32_t N = Pack<T>::N, kGroups = NT == 64 ? 4 : 1, kWaves = NT / 64, kFull = (1u << N) - 1u;
-  const uint32_t lane = threadIdx.x & 63u, group = NT == 64 ? threadIdx.x >> 6 : 0u, tid = NT == 64 ? lane : threadIdx.x;
+  const uint32_t group = NT == 64 ? threadIdx.x >> 6 : 0u;
   const uint32_t words = (a.K + 31u) / 32u;
   uint32_t* base = lds_words + group * distill_words(a.K, a.k, NT);
   const Entries en(base, a.k);
@@ -1034,6 +1043,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void distill_kernel(const Dist
   for (uint64_t row = (uint64_t)blockIdx.x * kGroups + group; row < a.n; row += (uint64_t)gridDim.x * kGroups) {
     const T* in = static_cast<const T*>(a.in) + row * a.stride;
     T* out = static_cast<T*>(a.grad) + row * a.grad_stride;
+    const uint32_t tid = forgotten(NT == 64 ? threadIdx.x & 63u : threadIdx.x), lane = tid & 63u;
     sync();  // the row before is done with the LDS
     for (uint32_t i = tid; i < words; i += NT) bitmap[i] = 0u;
     if (tid < 2u) ctl[tid] = 0u;
@@ -1230,8 +1240,9 @@ __global__ __launch_bounds__(256) void distill_thread_kernel(const DistillArgs a
   const double inv_T = 1.0 / a.temperature, x_scale = (double)c2;
   for (uint64_t r0 = (uint64_t)blockIdx.x * 256u; r0 < a.n; r0 += (uint64_t)gridDim.x * 256u) {
     const uint32_t rows = (uint32_t)(a.n - r0 < 256u ? a.n - r0 : 256u);
-    const bool active = threadIdx.x < rows;
-    const uint64_t row = r0 + threadIdx.x;
+    const uint32_t tid = forgotten(threadIdx.x);
+    const bool active = tid < rows;
+    const uint64_t row = r0 + tid;
     const int32_t* ids = a.ids + row * a.teacher_stride;
     const float* tv = a.values + row * a.teacher_stride;
     int32_t id[KK > 0 ? KK : 1];
@@ -1247,8 +1258,8 @@ __global__ __launch_bounds__(256) void distill_thread_kernel(const DistillArgs a
     stage_rows(static_cast<const T*>(a.in), r0, rows, a.K, a.stride, stage, pitch);
     __syncthreads();
     if (active) {
-      const T* x = stage + threadIdx.x * pitch;
-      float* g = gstage + threadIdx.x * gpitch;
+      const T* x = stage + tid * pitch;
+      float* g = gstage + tid * gpitch;
       auto each = [&](auto f) {  // f(entry, class, score) of the row's entries, in order
         if constexpr (KK > 0) {
 #pragma unroll
@@ -1332,7 +1343,7 @@ __global__ __launch_bounds__(256) void distill_thread_kernel(const DistillArgs a
         constexpr uint32_t N = Pack<T>::N;
         const uint32_t total = rows * a.K, magic = (uint32_t)((0x100000000ull + a.K - 1u) / a.K);
         T* dst = out + r0 * a.K;
-        for (uint32_t i = threadIdx.x * N; i < total; i += 256u * N) {
+        for (uint32_t i = tid * N; i < total; i += 256u * N) {
           uint32_t r = __umulhi(i, magic), c = i - r * a.K;
           float v[N];
 #pragma unroll
@@ -1344,8 +1355,8 @@ __global__ __launch_bounds__(256) void distill_thread_kernel(const DistillArgs a
           else store_pack<T>(dst, i, total, v);
         }
       } else {
-        for (uint32_t r = threadIdx.x >> 5; r < rows; r += 8u)
-          for (uint32_t c = threadIdx.x & 31u; c < a.K; c += 32u) out[(r0 + r) * a.grad_stride + c] = (T)gstage[r * gpitch + c];
+        for (uint32_t r = tid >> 5; r < rows; r += 8u)
+          for (uint32_t c = tid & 31u; c < a.K; c += 32u) out[(r0 + r) * a.grad_stride + c] = (T)gstage[r * gpitch + c];
       }
     }
   }
