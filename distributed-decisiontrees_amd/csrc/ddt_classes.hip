@@ -179,6 +179,8 @@ __device__ __forceinline__ F wave_sum(F v) {
   v += dpp<kRowBcast31, 0xC>((F)0, v);
   return last_lane(v);
 }
+// ... and over NT lanes of a row of scores: 16 (rotations within the row of lanes, every lane holds the result) or the whole wave
+constexpr int kRowRor1 = 0x121, kRowRor2 = 0x122, kRowRor4 = 0x124, kRowRor8 = 0x128;
 __device__ __forceinline__ float wave_max(float v) {
   v = fmaxf(v, dpp<kRowShr1, 0xF>(v, v));
   v = fmaxf(v, dpp<kRowShr2, 0xF>(v, v));
@@ -187,6 +189,25 @@ __device__ __forceinline__ float wave_max(float v) {
   v = fmaxf(v, dpp<kRowBcast15, 0xA>(v, v));
   v = fmaxf(v, dpp<kRowBcast31, 0xC>(v, v));
   return last_lane(v);
+}
+
+template <int NT, class F>
+__device__ __forceinline__ F lanes_sum(F v) {
+  if (NT != 16) return wave_sum(v);
+  v += dpp<kRowRor8, 0xF>((F)0, v);
+  v += dpp<kRowRor4, 0xF>((F)0, v);
+  v += dpp<kRowRor2, 0xF>((F)0, v);
+  v += dpp<kRowRor1, 0xF>((F)0, v);
+  return v;
+}
+template <int NT>
+__device__ __forceinline__ float lanes_max(float v) {
+  if (NT != 16) return wave_max(v);
+  v = fmaxf(v, dpp<kRowRor8, 0xF>(v, v));
+  v = fmaxf(v, dpp<kRowRor4, 0xF>(v, v));
+  v = fmaxf(v, dpp<kRowRor2, 0xF>(v, v));
+  v = fmaxf(v, dpp<kRowRor1, 0xF>(v, v));
+  return v;
 }
 
 // ---------------------------------------------------------------------------------------------------
@@ -446,16 +467,16 @@ struct RunSum {
     s += (t[0] + t[1]) + (t[2] + t[3]);
     return pm;
   }
-  // over the wave; plain(M) = this lane's sum of exp2((x - M) c)
-  template <class Plain>
+  // over the wave, or 16 lanes of it; plain(M) = this lane's sum of exp2((x - M) c)
+  template <int LANES, class Plain>
   __device__ __forceinline__ ExpSum finish(float c, Plain plain) const {
     ExpSum e;
-    e.m = wave_max(m);
+    e.m = lanes_max<LANES>(m);
     if (fabsf(e.m * c) <= kPlainBeyond) {
       const float R = reference(e.m, c);
-      e.s = wave_sum(s * exp2_fast(r - R)) * exp2_fast((float)fma((double)e.m, -(double)c, (double)R));
+      e.s = lanes_sum<LANES>(s * exp2_fast(r - R)) * exp2_fast((float)fma((double)e.m, -(double)c, (double)R));
     } else {
-      e.s = wave_sum(plain(e.m));
+      e.s = lanes_sum<LANES>(plain(e.m));
     }
     return e;
   }
@@ -782,7 +803,7 @@ __global__ __launch_bounds__(NT) void top_block_kernel(const TopArgs a) {
       chunk_done(-kInf);
     }
     const uint32_t best = score_key(run.m);  // (a thread without a candidate counts with the lowest score: the bound only sinks)
-    const ExpSum e = run.finish(c2, [&](float M) {
+    const ExpSum e = run.finish<64>(c2, [&](float M) {
       float t = 0.f;
       for (uint32_t p = tid; p < packs; p += NT) {
         float x[N];
@@ -958,35 +979,35 @@ struct Entries {
   static __host__ __device__ constexpr uint32_t words(uint32_t k) { return 7u * k; }
 };
 
-// one wave, one row: the teacher's entries against the student's row.  o = sums outside S.
-template <class T, bool GRAD>
+// one wave (or L = 16 lanes of it), one row: the teacher's entries against the student's row.  o = sums outside S.
+template <class T, int L, bool GRAD>
 __device__ __forceinline__ RowGrad row_loss(const DistillArgs& a, uint64_t row, const Entries& en, uint32_t lane, const ExpSum& o) {
   // the student's scale is the fp32 one of the sums outside S, for all its classes: p stays a softmax, of a temperature off by 2^-25
   const double inv_T = 1.0 / a.temperature, x_scale = (double)(float)(kLog2e / a.temperature);
   constexpr double kLn2 = 0.69314718055994530942;
   float xm = -FLT_MAX, tm = -FLT_MAX;
-  for (uint32_t j = lane; j < a.k; j += 64u)
+  for (uint32_t j = lane; j < a.k; j += L)
     if (en.id[j] >= 0) xm = fmaxf(xm, en.x[j]), tm = fmaxf(tm, en.t[j]);
-  const float M = wave_max(fmaxf(xm, o.m));
-  tm = wave_max(tm);
+  const float M = lanes_max<L>(fmaxf(xm, o.m));
+  tm = lanes_max<L>(tm);
   const double shift = a.lse ? (double)a.lse[row] : (double)tm * inv_T;
   double zs = 0.0, ts = 0.0;
-  for (uint32_t j = lane; j < a.k; j += 64u)
+  for (uint32_t j = lane; j < a.k; j += L)
     if (en.id[j] >= 0) {
       const double e = exp2_64(((double)en.x[j] - (double)M) * x_scale), q = exp2_64(((double)en.t[j] * inv_T - shift) * kLog2e);
       en.e[j] = e, en.q[j] = q;
       ts += q;
       if (!(en.id[j] & kAgain)) zs += e;
     }
-  zs = wave_sum(zs), ts = wave_sum(ts);
+  zs = lanes_sum<L>(zs), ts = lanes_sum<L>(ts);
   const double far = exp2_64(((double)o.m - (double)M) * x_scale), Z = (double)o.s * far + zs, log_Z = log_64(Z);
   // without lse the q are still to be divided by their sum
   const double log_T = a.lse ? shift : shift + log_64(ts), scale = a.lse ? 1.0 : 1.0 / ts;
   double Q = a.lse ? ts : 1.0, rest = 0.0, loss = 0.0;
-  for (uint32_t j = lane; j < a.k; j += 64u)
+  for (uint32_t j = lane; j < a.k; j += L)
     if (en.id[j] >= 0 && !(en.q[j] == 0.0))
       loss += en.q[j] * scale * (((double)en.t[j] * inv_T - log_T) - (((double)en.x[j] - (double)M) * x_scale * kLn2 - log_Z));
-  loss = wave_sum(loss);
+  loss = lanes_sum<L>(loss);
   if (a.lse && o.s > 0.f && Q < 1.0) {
     rest = 1.0 - Q;
     loss += rest * (log_64(rest) - (((double)o.m - (double)M) * x_scale * kLn2 + log_64((double)o.s) - log_Z));
@@ -999,7 +1020,7 @@ __device__ __forceinline__ RowGrad row_loss(const DistillArgs& a, uint64_t row, 
     // (nothing outside S: no gradient there; nothing in the whole row: NaN, as its softmax)
     g.coef = !(o.s == 0.f) ? (float)((Q * far / Z - rest / (double)o.s) * w) : Z == 0.0 ? __builtin_nanf("") : 0.f;
     T* out = static_cast<T*>(a.grad) + row * a.grad_stride;
-    for (uint32_t j = lane; j < a.k; j += 64u) {
+    for (uint32_t j = lane; j < a.k; j += L) {
       const int32_t id = en.id[j];
       if (id < 0 || (id & kAgain)) continue;
       double qc = en.q[j];
@@ -1012,17 +1033,17 @@ __device__ __forceinline__ RowGrad row_loss(const DistillArgs& a, uint64_t row, 
 }
 
 __host__ __device__ constexpr uint32_t distill_words(uint32_t K, uint32_t k, uint32_t threads) {  // LDS of a row, an even number
-  return (Entries::words(k) + 4u + 2u * (threads / 64u) + (K + 31u) / 32u + 1u) & ~1u;
+  return (Entries::words(k) + 4u + 2u * ((threads + 63u) / 64u) + (K + 31u) / 32u + 1u) & ~1u;
 }
 
-// NT threads per row: 64 (a wave; 4 rows per block of 256) or the whole block.  P > 0: the row's packs stay in registers, P per thread,
+// NT threads per row: 16 (4 rows per wave: what a row does once costs a fourth of a wave), 64 (a wave) or the whole block.  P > 0: the row's packs stay in registers, P per thread,
 // all of them loaded at once while the teacher's entries are fetched, so that the gradient costs one read and one write of the matrix.
 // P = 0 (rows of more than 512 x 32 packs): the row is read a second time for the gradient, from whichever cache still holds it.
 // S is a bitmap in LDS, a pack's bits next to each other.
 template <class T, int NT, int P, bool GRAD>
-__global__ __launch_bounds__(NT == 64 ? 256 : NT) void distill_kernel(const DistillArgs a) {
-  constexpr uint32_t N = Pack<T>::N, kGroups = NT == 64 ? 4 : 1, kWaves = NT / 64, kFull = (1u << N) - 1u;
-  const uint32_t group = NT == 64 ? threadIdx.x >> 6 : 0u;
+__global__ __launch_bounds__(NT < 256 ? 256 : NT) void distill_kernel(const DistillArgs a) {
+  constexpr uint32_t N = Pack<T>::N, kGroups = NT < 256 ? 256 / NT : 1, kWaves = (NT + 63) / 64, kFull = (1u << N) - 1u;
+  const uint32_t group = NT < 256 ? threadIdx.x / NT : 0u;
   const uint32_t words = (a.K + 31u) / 32u;
   uint32_t* base = lds_words + group * distill_words(a.K, a.k, NT);
   const Entries en(base, a.k);
@@ -1032,7 +1053,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void distill_kernel(const Dist
   const uint32_t packs = (a.K + N - 1u) / N;
   const float c2 = (float)(kLog2e / a.temperature);
   auto sync = [] {
-    if (NT == 64) {
+    if (NT <= 64) {
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
     } else {
@@ -1043,12 +1064,12 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void distill_kernel(const Dist
   for (uint64_t row = (uint64_t)blockIdx.x * kGroups + group; row < a.n; row += (uint64_t)gridDim.x * kGroups) {
     const T* in = static_cast<const T*>(a.in) + row * a.stride;
     T* out = static_cast<T*>(a.grad) + row * a.grad_stride;
-    const uint32_t tid = forgotten(NT == 64 ? threadIdx.x & 63u : threadIdx.x), lane = tid & 63u;
+    const uint32_t tid = forgotten(NT < 256 ? threadIdx.x % NT : threadIdx.x), lane = tid & 63u;
     sync();  // the row before is done with the LDS
     for (uint32_t i = tid; i < words; i += NT) bitmap[i] = 0u;
     if (tid < 2u) ctl[tid] = 0u;
     // a block's thread fetches one entry and its score of the student itself: ahead of the row, which the score is read behind
-    static_assert(NT == 64 || NT >= DDT_MAX_TOP, "an entry per thread");
+    static_assert(NT <= 64 || NT >= DDT_MAX_TOP, "an entry per thread");
     int32_t my_id = -1;
     float my_t = 0.f, my_x = 0.f;
     if (NT > 64 && tid < a.k) my_id = a.ids[row * a.teacher_stride + tid], my_t = a.values[row * a.teacher_stride + tid];
@@ -1142,7 +1163,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void distill_kernel(const Dist
         run.add(x, c2);
       }
     }
-    ExpSum o = run.finish(c2, [&](float M) {
+    ExpSum o = run.template finish<NT < 64 ? NT : 64>(c2, [&](float M) {
       float t = 0.f;
       for (uint32_t p = tid; p < packs; p += NT) {
         float x[N];
@@ -1163,7 +1184,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void distill_kernel(const Dist
         o.m = lane < kWaves ? part[2 * lane] : -FLT_MAX, o.s = lane < kWaves ? part[2 * lane + 1] : 0.f;
         o.reduce_wave(c2);
       }
-      const RowGrad g = row_loss<T, GRAD>(a, row, en, lane, o);
+      const RowGrad g = row_loss<T, (NT < 64 ? NT : 64), GRAD>(a, row, en, lane, o);
       if (GRAD && lane == 0u) ctl[2] = __float_as_uint(g.m), ctl[3] = __float_as_uint(g.coef);
     }
     if (GRAD) {
@@ -1451,9 +1472,9 @@ hipError_t top_typed(const TopArgs& a, bool class_major, hipStream_t s) {
 
 template <class T, int NT, int P, bool GRAD>
 hipError_t distill_rows(const DistillArgs& a, hipStream_t s) {
-  constexpr uint32_t groups = NT == 64 ? 4u : 1u;
+  constexpr uint32_t groups = NT < 256 ? 256u / NT : 1u;
   const uint32_t lds = groups * 4u * distill_words(a.K, a.k, NT);
-  return launch(distill_kernel<T, NT, P, GRAD>, (a.n + groups - 1) / groups, NT == 64 ? 256 : NT, lds, s, a);
+  return launch(distill_kernel<T, NT, P, GRAD>, (a.n + groups - 1) / groups, NT < 256 ? 256 : NT, lds, s, a);
 }
 template <class T, bool GRAD>
 hipError_t distill_typed(const DistillArgs& a, hipStream_t s) {
@@ -1472,6 +1493,16 @@ hipError_t distill_typed(const DistillArgs& a, hipStream_t s) {
     }
   }
   const uint32_t packs = (a.K + Pack<T>::N - 1) / Pack<T>::N;
+  // Short rows: what a row does once (its 64-bit numbers, its reductions) outweighs its scores, so four of them share a wave -- where there
+  // are rows enough to fill the chip that way.  (100 M scores, us, 64 -> 16 threads per row: loss + gradient of 200 bf16 classes 922 -> 333,
+  // 500 fp32 386 -> 271, 1500 bf16 212 -> 171; 1000 fp32 239 -> 258.)
+  if (a.n >= 4096u && a.k <= 64u && packs <= 256u) {
+    if (packs <= 16u) return distill_rows<T, 16, 1, GRAD>(a, s);
+    if (packs <= 32u) return distill_rows<T, 16, 2, GRAD>(a, s);
+    if (packs <= 64u) return distill_rows<T, 16, 4, GRAD>(a, s);
+    if (packs <= 128u) return distill_rows<T, 16, 8, GRAD>(a, s);
+    return distill_rows<T, 16, 16, GRAD>(a, s);
+  }
   if (packs <= 64u) return distill_rows<T, 64, 1, GRAD>(a, s);
   if (packs <= 128u) return distill_rows<T, 64, 2, GRAD>(a, s);
   if (packs <= 256u) return distill_rows<T, 64, 4, GRAD>(a, s);
@@ -1480,9 +1511,9 @@ hipError_t distill_typed(const DistillArgs& a, hipStream_t s) {
   // packs -- for the gradient no more than keep their rows in the 256 MB cache until their second read.  (200 M scores, us, 256 / 512 /
   // 1024 threads: loss of 50257 fp16-sized classes 89 / 109 / 143; gradient 64000 bf16 253 / 249 / 319, 100000 fp32 516 / 454 / 397.)
   if (a.n <= 512u) return distill_rows<T, 1024, 0, GRAD>(a, s);
-  if (!GRAD) return distill_rows<T, 256, 0, GRAD>(a, s);
+  if (!GRAD) return packs <= 1024u ? distill_rows<T, 256, 4, GRAD>(a, s) : distill_rows<T, 256, 0, GRAD>(a, s);
   if (packs <= 1024u) return distill_rows<T, 256, 4, GRAD>(a, s);
-  if (packs <= 2048u) return distill_rows<T, 256, 8, GRAD>(a, s);
+  if (packs <= 3072u) return distill_rows<T, 256, 0, GRAD>(a, s);
   if (packs <= 4096u) return distill_rows<T, 256, 16, GRAD>(a, s);
   return packs <= 16384u ? distill_rows<T, 512, 0, GRAD>(a, s) : distill_rows<T, 1024, 0, GRAD>(a, s);
 }

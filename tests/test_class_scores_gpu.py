@@ -411,7 +411,7 @@ def check_distill(engine, x, ids, vals, lse, T, w=None, grad_out=None):
     return loss, g
 
 
-DISTILL = [(1, 1, 1), (3, 2, 2), (700, 10, 4), (257, 32, 40), (5, 33, 33), (6, 200, 256), (64, 1000, 16), (3, 2048, 65), (4, 2049, 50), (3, 5003, 256),
+DISTILL = [(1, 1, 1), (3, 2, 2), (700, 10, 4), (257, 32, 40), (5, 33, 33), (6, 200, 256), (64, 1000, 16), (5000, 40, 3), (4097, 130, 64), (4100, 300, 65), (4096, 515, 20), (3, 2048, 65), (4, 2049, 50), (3, 5003, 256),
            (3, 16385, 64), (3, 50257, 256), (1, 131072, 1), (1, 1 << 20, 100)]
 
 
