@@ -156,6 +156,10 @@ __device__ __forceinline__ float dpp(float idle, float v) {
   return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp((int)__float_as_uint(idle), (int)__float_as_uint(v), CTRL, ROWS, 0xF, false));
 }
 template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp(uint32_t idle, uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp((int)idle, (int)v, CTRL, ROWS, 0xF, false);
+}
+template <int CTRL, int ROWS>
 __device__ __forceinline__ double dpp(double idle, double v) {
   const uint64_t i = (uint64_t)__double_as_longlong(idle), b = (uint64_t)__double_as_longlong(v);
   const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp((int)(uint32_t)i, (int)(uint32_t)b, CTRL, ROWS, 0xF, false);
@@ -623,6 +627,118 @@ __device__ __forceinline__ uint32_t rank_of(uint64_t mine, const uint64_t* list,
 #pragma unroll 8
   for (uint32_t j = 0; j < count; ++j) rank += list[j] > mine;
   return rank;
+}
+
+// few classes, more than 8 of them wanted: a thread per row, every class's rank counted against the others'.  For c < d one comparison
+// serves both: g = x_d > x_c puts d before c, otherwise c, the lower class, stands first.  KP >= K classes in registers.
+template <class T, bool CM, int KP>
+__global__ __launch_bounds__(256) void top_rank_kernel(const TopArgs a) {
+  T* stage = reinterpret_cast<T*>(lds_words);
+  const uint32_t pitch = staged_pitch<T>(a.K), columns = a.k < a.K ? a.k : a.K, opitch = columns | 1u;
+  float* out_value = reinterpret_cast<float*>(lds_words);  // (takes the place of the staged rows, which are in registers by then)
+  int32_t* out_id = reinterpret_cast<int32_t*>(lds_words + 256u * opitch);
+  const float c2 = (float)(kLog2e / a.temperature);
+  for (uint64_t r0 = (uint64_t)blockIdx.x * 256u; r0 < a.n; r0 += (uint64_t)gridDim.x * 256u) {
+    const uint32_t rows = (uint32_t)(a.n - r0 < 256u ? a.n - r0 : 256u), tid = forgotten(threadIdx.x);
+    const T* in = static_cast<const T*>(a.in);
+    const bool active = tid < rows;
+    __syncthreads();
+    if (!CM) {
+      stage_rows(in, r0, rows, a.K, a.stride, stage, pitch);
+      __syncthreads();
+    }
+    float x[KP];
+    if (active) {
+#pragma unroll
+      for (uint32_t c = 0; c < KP; ++c) x[c] = c < a.K ? (float)(CM ? in[c * a.stride + r0 + tid] : stage[tid * pitch + c]) : -kInf;
+    }
+    __syncthreads();
+    if (active) {
+      ExpSum e;
+#pragma unroll
+      for (int c = 0; c < KP; ++c) e.m = fmaxf(e.m, x[c]);
+#pragma unroll
+      for (int c = 0; c < KP; ++c) {
+        e.s += exp2_fast((x[c] - e.m) * c2);
+        x[c] = x[c] > -kInf ? x[c] : -kInf;  // (NaN is no candidate)
+      }
+      if (a.lse) a.lse[r0 + tid] = log_sum(e, 1.0 / a.temperature);
+      uint32_t rank[KP];
+#pragma unroll
+      for (int c = 0; c < KP; ++c) rank[c] = c;
+#pragma unroll
+      for (int c = 0; c < KP; ++c)
+#pragma unroll
+        for (int d = c + 1; d < KP; ++d) {
+          const bool g = x[d] > x[c];
+          rank[c] += g, rank[d] -= g;
+        }
+      float* ov = out_value + tid * opitch;
+      int32_t* oi = out_id + tid * opitch;
+      for (uint32_t j = 0; j < columns; ++j) ov[j] = -kInf, oi[j] = -1;
+#pragma unroll
+      for (int c = 0; c < KP; ++c)
+        if (x[c] > -kInf && rank[c] < columns) ov[rank[c]] = x[c], oi[rank[c]] = c;
+    }
+    __syncthreads();
+    const uint32_t total = rows * a.k, magic = 0xFFFFFFFFu / a.k + 1u;  // (total k < 2^32, k > 8)
+    for (uint32_t i = tid; i < total; i += 256u) {
+      const uint32_t r = __umulhi(i, magic), j = i - r * a.k;
+      a.ids[r0 * a.k + i] = j < columns ? out_id[r * opitch + j] : -1;
+      a.values[r0 * a.k + i] = j < columns ? out_value[r * opitch + j] : -kInf;
+    }
+  }
+}
+
+// short rows, few classes wanted: 16 lanes per row, P packs per lane in registers; the best is taken out k times, lane j keeps the j-th.
+template <class T, int P>
+__global__ __launch_bounds__(256) void top_lanes_kernel(const TopArgs a) {
+  constexpr int N = (int)Pack<T>::N, E = P * N;
+  const float c2 = (float)(kLog2e / a.temperature);
+  for (uint64_t row = (uint64_t)blockIdx.x * 16u + (threadIdx.x >> 4); row < a.n; row += (uint64_t)gridDim.x * 16u) {
+    const uint32_t lane = forgotten(threadIdx.x & 15u);
+    float x[E], best = -kInf;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      float v[N];
+      load_pack(static_cast<const T*>(a.in) + row * a.stride, ((uint32_t)p * 16u + lane) * N, a.K, -kInf, v);
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[p * N + i] = v[i], best = fmaxf(best, v[i]);
+    }
+    ExpSum e;
+    e.m = fmaxf(lanes_max<16>(best), -FLT_MAX);
+#pragma unroll
+    for (int i = 0; i < E; ++i) e.s += exp2_fast((x[i] - e.m) * c2);
+    e.s = lanes_sum<16>(e.s);
+    if (a.lse && lane == 0u) a.lse[row] = log_sum(e, 1.0 / a.temperature);
+    float value = -kInf;
+    int32_t id = -1;
+    for (uint32_t j = 0; j < a.k; ++j) {
+      float b = -kInf;
+      uint32_t at = 0xFFFFFFFFu;
+#pragma unroll
+      for (int i = 0; i < E; ++i) {  // (in the order of the classes; NaN and -inf are never better)
+        const bool g = x[i] > b;
+        b = g ? x[i] : b, at = g ? (uint32_t)i : at;
+      }
+      const uint32_t mine = at == 0xFFFFFFFFu ? at : (at / N * 16u + lane) * N + at % N;
+      uint32_t c = mine;
+      auto meet = [&](float ob, uint32_t oc) {
+        const bool g = ob > b || (ob == b && oc < c);
+        b = g ? ob : b, c = g ? oc : c;
+      };
+      meet(dpp<kRowRor8, 0xF>(b, b), dpp<kRowRor8, 0xF>(c, c));
+      meet(dpp<kRowRor4, 0xF>(b, b), dpp<kRowRor4, 0xF>(c, c));
+      meet(dpp<kRowRor2, 0xF>(b, b), dpp<kRowRor2, 0xF>(c, c));
+      meet(dpp<kRowRor1, 0xF>(b, b), dpp<kRowRor1, 0xF>(c, c));
+      if (lane == j) value = b, id = (int32_t)c;  // (nothing left: -inf and -1)
+      if (c == mine) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) x[i] = (uint32_t)i == at ? -kInf : x[i];
+      }
+    }
+    if (lane < a.k) a.ids[row * a.k + lane] = id, a.values[row * a.k + lane] = value;
+  }
 }
 
 // up to 2048 classes: a wave per row, all its keys in registers (P packs per lane).  Class-major rows are staged through LDS, 16 at a
@@ -1461,10 +1577,31 @@ template <class T, int NT>
 hipError_t top_block(const TopArgs& a, hipStream_t s) {
   return launch(top_block_kernel<T, NT>, a.n, NT, 4u * top_block_words(NT), s, a);
 }
+template <class T, bool CM>
+hipError_t top_rank(const TopArgs& a, hipStream_t s) {
+  constexpr uint32_t per_word = 4 / sizeof(T);
+  const uint32_t staged = CM ? 0u : 256u * (uint32_t)sizeof(T) * ((((a.K + per_word - 1) / per_word) | 1u) * per_word);
+  const uint32_t out = 256u * 8u * ((a.k < a.K ? a.k : a.K) | 1u), lds = staged > out ? staged : out;
+  const uint64_t blocks = (a.n + 255) / 256;
+  return a.K <= 16u ? launch(top_rank_kernel<T, CM, 16>, blocks, 256, lds, s, a) : launch(top_rank_kernel<T, CM, 32>, blocks, 256, lds, s, a);
+}
 template <class T>
 hipError_t top_typed(const TopArgs& a, bool class_major, hipStream_t s) {
-  if (a.K <= 32u && a.k <= 8u) return class_major ? top_thread<T, true>(a, s) : top_thread<T, false>(a, s);
+  constexpr uint32_t N = Pack<T>::N;
+  if (a.K <= 32u && a.k > 8u) return class_major ? top_rank<T, true>(a, s) : top_rank<T, false>(a, s);
+  // a thread per row reads class-major rows as they lie; with many classes it takes many rows to fill the chip
+  if (class_major && a.k <= 8u && (a.K <= 32u || a.n >= 65536u)) return top_thread<T, true>(a, s);
+  if (a.K <= 32u) return top_thread<T, false>(a, s);
   if (class_major) return a.K <= kTopMaxClassMajor ? top_wave<T, true>(a, s) : hipErrorInvalidValue;
+  // 16 lanes per row take out the best k times, 5 instructions per score and 40 each: against about 600 per row for a whole wave
+  const uint32_t packs = (a.K + N - 1) / N, p = packs <= 16u ? 1u : packs <= 32u ? 2u : packs <= 64u ? 4u : 8u;
+  if (a.n >= 4096u && a.k <= 16u && packs <= 512u / N && a.k * (5u * p * N + 40u) <= 2400u) {
+    const uint64_t blocks = (a.n + 15) / 16;
+    if (p == 1u) return launch(top_lanes_kernel<T, 1>, blocks, 256, 0, s, a);
+    if (p == 2u) return launch(top_lanes_kernel<T, 2>, blocks, 256, 0, s, a);
+    if (p == 4u) return launch(top_lanes_kernel<T, 4>, blocks, 256, 0, s, a);
+    if constexpr (N == 4) return launch(top_lanes_kernel<T, 8>, blocks, 256, 0, s, a);
+  }
   if (a.K <= 2048u) return top_wave<T, false>(a, s);
   if (a.K <= 16384u) return top_block<T, 256>(a, s);
   return a.n > 256u ? top_block<T, 512>(a, s) : top_block<T, 1024>(a, s);
