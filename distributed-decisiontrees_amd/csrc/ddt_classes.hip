@@ -524,7 +524,7 @@ __device__ __forceinline__ uint32_t staged_pitch(uint32_t K) {  // elements
 }
 template <class T>
 __device__ __forceinline__ void stage_rows(const T* in, uint64_t r0, uint32_t rows, uint32_t K, uint64_t stride, T* dst, uint32_t pitch) {
-  if (stride == K) {  // one piece of rows * K scores (at most 256 * 32)
+  if (stride == K) {  // one piece of rows * K scores (at most 256 * 64)
     const T* src = in + r0 * K;
     const uint32_t total = rows * K, magic = (uint32_t)((0x100000000ull + K - 1u) / K);  // K >= 2: i / K = umulhi(i, magic) for i < 2^16
     constexpr uint32_t N = Pack<T>::N;
@@ -690,18 +690,49 @@ __global__ __launch_bounds__(256) void top_rank_kernel(const TopArgs a) {
   }
 }
 
+// class-major rows [r0, r0 + 16) into stage[class][17] as fp32: 64-byte pieces (of fp32) out of every class's vector; with 17 words per class
+// neither the writes nor reads by consecutive lanes of consecutive classes meet in a bank
+constexpr uint32_t kStagePitch = 17;
+template <class T>
+__device__ __forceinline__ void stage_class_major(const TopArgs& a, uint64_t r0, float* stage) {
+  constexpr uint32_t N = Pack<T>::N, kPieces = 16u / N;
+  const uint32_t rows = (uint32_t)(a.n - r0 < 16u ? a.n - r0 : 16u), q = threadIdx.x % kPieces * N;
+  for (uint32_t c = threadIdx.x / kPieces; c < a.K; c += blockDim.x / kPieces) {
+    float v[N];
+    load_pack(static_cast<const T*>(a.in) + c * a.stride + r0, q, rows, 0.f, v);
+#pragma unroll
+    for (uint32_t i = 0; i < N; ++i) stage[c * kStagePitch + q + i] = v[i];
+  }
+}
+
 // short rows, few classes wanted: 16 lanes per row, P packs per lane in registers; the best is taken out k times, lane j keeps the j-th.
-template <class T, int P>
+template <class T, bool CM, int P>
 __global__ __launch_bounds__(256) void top_lanes_kernel(const TopArgs a) {
   constexpr int N = (int)Pack<T>::N, E = P * N;
+  float* stage = reinterpret_cast<float*>(lds_words);
   const float c2 = (float)(kLog2e / a.temperature);
-  for (uint64_t row = (uint64_t)blockIdx.x * 16u + (threadIdx.x >> 4); row < a.n; row += (uint64_t)gridDim.x * 16u) {
+  for (uint64_t r0 = (uint64_t)blockIdx.x * 16u; r0 < a.n; r0 += (uint64_t)gridDim.x * 16u) {
+    if (CM) {
+      __syncthreads();
+      stage_class_major<T>(a, r0, stage);
+      __syncthreads();
+    }
+    const uint64_t row = r0 + (threadIdx.x >> 4);
+    if (row >= a.n) continue;
     const uint32_t lane = forgotten(threadIdx.x & 15u);
     float x[E], best = -kInf;
 #pragma unroll
     for (int p = 0; p < P; ++p) {
       float v[N];
-      load_pack(static_cast<const T*>(a.in) + row * a.stride, ((uint32_t)p * 16u + lane) * N, a.K, -kInf, v);
+      if (CM) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const uint32_t c = (uint32_t)(p * N + i) * 16u + lane;
+          v[i] = c < a.K ? stage[c * kStagePitch + (threadIdx.x >> 4)] : -kInf;
+        }
+      } else {
+        load_pack(static_cast<const T*>(a.in) + row * a.stride, ((uint32_t)p * 16u + lane) * N, a.K, -kInf, v);
+      }
 #pragma unroll
       for (int i = 0; i < N; ++i) x[p * N + i] = v[i], best = fmaxf(best, v[i]);
     }
@@ -721,7 +752,7 @@ __global__ __launch_bounds__(256) void top_lanes_kernel(const TopArgs a) {
         const bool g = x[i] > b;
         b = g ? x[i] : b, at = g ? (uint32_t)i : at;
       }
-      const uint32_t mine = at == 0xFFFFFFFFu ? at : (at / N * 16u + lane) * N + at % N;
+      const uint32_t mine = at == 0xFFFFFFFFu ? at : CM ? at * 16u + lane : (at / N * 16u + lane) * N + at % N;
       uint32_t c = mine;
       auto meet = [&](float ob, uint32_t oc) {
         const bool g = ob > b || (ob == b && oc < c);
@@ -742,7 +773,7 @@ __global__ __launch_bounds__(256) void top_lanes_kernel(const TopArgs a) {
 }
 
 // up to 2048 classes: a wave per row, all its keys in registers (P packs per lane).  Class-major rows are staged through LDS, 16 at a
-// time (64-byte pieces of fp32), for the 8 waves of the block.
+// time for the 8 waves of the block.
 constexpr uint32_t kWaveList = 128;  // candidates that are ranked without an exact count
 __device__ __forceinline__ uint32_t lanes_below(uint64_t ballot) {
   return __builtin_amdgcn_mbcnt_hi((uint32_t)(ballot >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)ballot, 0u));
@@ -756,30 +787,28 @@ __global__ __launch_bounds__(top_wave_waves(CM) * 64) void top_wave_kernel(const
   constexpr uint32_t kRows = top_wave_rows(CM), kWaves = top_wave_waves(CM);
   const uint32_t wave = threadIdx.x >> 6;
   uint64_t* list = reinterpret_cast<uint64_t*>(lds_words) + wave * wave_list(a.k);  // the wave's selected candidates
-  T* stage = reinterpret_cast<T*>(reinterpret_cast<uint64_t*>(lds_words) + kWaves * wave_list(a.k));  // class-major: [K][16] scores
+  float* stage = reinterpret_cast<float*>(reinterpret_cast<uint64_t*>(lds_words) + kWaves * wave_list(a.k));  // class-major
   const float c2 = (float)(kLog2e / a.temperature);
   for (uint64_t r0 = (uint64_t)blockIdx.x * kRows; r0 < a.n; r0 += (uint64_t)gridDim.x * kRows) {
     if (CM) {
       __syncthreads();
-      const uint32_t r = threadIdx.x & 15u;
-      if (r0 + r < a.n)
-        for (uint32_t c = threadIdx.x >> 4; c < a.K; c += kWaves * 4u) stage[c * 16u + r] = static_cast<const T*>(a.in)[c * a.stride + r0 + r];
+      stage_class_major<T>(a, r0, stage);
       __syncthreads();
     }
     for (uint32_t rr = wave; rr < kRows && r0 + rr < a.n; rr += kWaves) {
       const uint64_t row = r0 + rr;
       const uint32_t lane = forgotten(threadIdx.x & 63u);
+      auto class_of = [&](int i) { return CM ? (uint32_t)i * 64u + lane : ((uint32_t)(i / N) * 64u + lane) * N + i % N; };
       float x[E];
       float best = -kInf;
 #pragma unroll
       for (int p = 0; p < P; ++p) {
-        const uint32_t c = ((uint32_t)p * 64u + lane) * N;
         float v[N];
         if (CM) {
 #pragma unroll
-          for (int i = 0; i < N; ++i) v[i] = c + i < a.K ? (float)stage[(c + i) * 16u + rr] : -kInf;
+          for (int i = 0; i < N; ++i) v[i] = class_of(p * N + i) < a.K ? stage[class_of(p * N + i) * kStagePitch + rr] : -kInf;
         } else {
-          load_pack(static_cast<const T*>(a.in) + row * a.stride, c, a.K, -kInf, v);
+          load_pack(static_cast<const T*>(a.in) + row * a.stride, class_of(p * N), a.K, -kInf, v);
         }
 #pragma unroll
         for (int i = 0; i < N; ++i) x[p * N + i] = v[i], best = fmaxf(best, v[i]);
@@ -803,7 +832,7 @@ __global__ __launch_bounds__(top_wave_waves(CM) * 64) void top_wave_kernel(const
           const bool take = x[i] >= bound;
           const uint64_t b = __ballot(take);
           const uint32_t slot = count + lanes_below(b);
-          if (take && slot < kWaveList) list[slot] = candidate(score_key(x[i]), ((uint32_t)(i / N) * 64u + lane) * N + i % N);
+          if (take && slot < kWaveList) list[slot] = candidate(score_key(x[i]), class_of(i));
           count += __popcll(b);
         }
       }
@@ -828,7 +857,7 @@ __global__ __launch_bounds__(top_wave_waves(CM) * 64) void top_wave_kernel(const
             uint32_t cnt = gt;
 #pragma unroll
             for (int i = 0; i < E; ++i) {
-              const uint32_t c = ((uint32_t)(i / N) * 64u + lane) * N + i % N;
+              const uint32_t c = class_of(i);
               cnt += __popcll(__ballot(key[i] >= t && key[i] < above && c < cand));
             }
             if (cnt < kk) last = cand;
@@ -837,7 +866,7 @@ __global__ __launch_bounds__(top_wave_waves(CM) * 64) void top_wave_kernel(const
         count = 0u;
 #pragma unroll
         for (int i = 0; i < E; ++i) {
-          const uint32_t c = ((uint32_t)(i / N) * 64u + lane) * N + i % N;
+          const uint32_t c = class_of(i);
           const bool take = key[i] >= t && (key[i] >= above || c <= last);
           const uint64_t b = __ballot(take);
           if (take) list[count + lanes_below(b)] = candidate(key[i], c);
@@ -1566,7 +1595,7 @@ template <class T, bool CM>
 hipError_t top_wave(const TopArgs& a, hipStream_t s) {
   constexpr uint32_t N = Pack<T>::N, rows = top_wave_rows(CM), threads = top_wave_waves(CM) * 64u;
   const uint64_t blocks = (a.n + rows - 1) / rows;
-  const uint32_t lds = top_wave_waves(CM) * wave_list(a.k) * 8u + (CM ? a.K * 16u * (uint32_t)sizeof(T) : 0u), packs = (a.K + N - 1) / N;
+  const uint32_t lds = top_wave_waves(CM) * wave_list(a.k) * 8u + (CM ? a.K * kStagePitch * 4u : 0u), packs = (a.K + N - 1) / N;
   if (packs <= 64u) return launch(top_wave_kernel<T, CM, 1>, blocks, threads, lds, s, a);
   if (packs <= 128u) return launch(top_wave_kernel<T, CM, 2>, blocks, threads, lds, s, a);
   if (packs <= 256u) return launch(top_wave_kernel<T, CM, 4>, blocks, threads, lds, s, a);
@@ -1585,23 +1614,29 @@ hipError_t top_rank(const TopArgs& a, hipStream_t s) {
   const uint64_t blocks = (a.n + 255) / 256;
   return a.K <= 16u ? launch(top_rank_kernel<T, CM, 16>, blocks, 256, lds, s, a) : launch(top_rank_kernel<T, CM, 32>, blocks, 256, lds, s, a);
 }
+template <class T, bool CM>
+hipError_t top_lanes(const TopArgs& a, uint32_t p, hipStream_t s) {
+  const uint64_t blocks = (a.n + 15) / 16;
+  const uint32_t lds = CM ? a.K * kStagePitch * 4u : 0u;
+  if (p == 1u) return launch(top_lanes_kernel<T, CM, 1>, blocks, 256, lds, s, a);
+  if (p == 2u) return launch(top_lanes_kernel<T, CM, 2>, blocks, 256, lds, s, a);
+  if (p == 4u) return launch(top_lanes_kernel<T, CM, 4>, blocks, 256, lds, s, a);
+  if constexpr (Pack<T>::N == 4) return launch(top_lanes_kernel<T, CM, 8>, blocks, 256, lds, s, a);
+  return hipErrorInvalidValue;
+}
 template <class T>
 hipError_t top_typed(const TopArgs& a, bool class_major, hipStream_t s) {
   constexpr uint32_t N = Pack<T>::N;
   if (a.K <= 32u && a.k > 8u) return class_major ? top_rank<T, true>(a, s) : top_rank<T, false>(a, s);
   // a thread per row reads class-major rows as they lie; with many classes it takes many rows to fill the chip
   if (class_major && a.k <= 8u && (a.K <= 32u || a.n >= 65536u)) return top_thread<T, true>(a, s);
-  if (a.K <= 32u) return top_thread<T, false>(a, s);
-  if (class_major) return a.K <= kTopMaxClassMajor ? top_wave<T, true>(a, s) : hipErrorInvalidValue;
+  if (!class_major && a.k <= 8u && (a.K <= 32u || (a.K <= 64u && a.n >= 65536u))) return top_thread<T, false>(a, s);
+  if (class_major && a.K > kTopMaxClassMajor) return hipErrorInvalidValue;
   // 16 lanes per row take out the best k times, 5 instructions per score and 40 each: against about 600 per row for a whole wave
   const uint32_t packs = (a.K + N - 1) / N, p = packs <= 16u ? 1u : packs <= 32u ? 2u : packs <= 64u ? 4u : 8u;
-  if (a.n >= 4096u && a.k <= 16u && packs <= 512u / N && a.k * (5u * p * N + 40u) <= 2400u) {
-    const uint64_t blocks = (a.n + 15) / 16;
-    if (p == 1u) return launch(top_lanes_kernel<T, 1>, blocks, 256, 0, s, a);
-    if (p == 2u) return launch(top_lanes_kernel<T, 2>, blocks, 256, 0, s, a);
-    if (p == 4u) return launch(top_lanes_kernel<T, 4>, blocks, 256, 0, s, a);
-    if constexpr (N == 4) return launch(top_lanes_kernel<T, 8>, blocks, 256, 0, s, a);
-  }
+  if (a.n >= 4096u && a.k <= 16u && packs <= 512u / N && a.k * (5u * p * N + 40u) <= 2400u)
+    return class_major ? top_lanes<T, true>(a, p, s) : top_lanes<T, false>(a, p, s);
+  if (class_major) return top_wave<T, true>(a, s);
   if (a.K <= 2048u) return top_wave<T, false>(a, s);
   if (a.K <= 16384u) return top_block<T, 256>(a, s);
   return a.n > 256u ? top_block<T, 512>(a, s) : top_block<T, 1024>(a, s);

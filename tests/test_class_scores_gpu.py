@@ -255,7 +255,7 @@ def values_equal(a, b):
 TOP = [(1, 1, 1), (3, 2, 2), (300, 10, 3), (1000, 32, 8), (257, 32, 9), (70, 33, 1), (5, 200, 256), (17, 513, 64), (33, 1000, 20), (4, 1025, 200),
        (2, 2047, 256), (3, 2048, 5), (3, 2049, 50), (4, 5000, 256), (2, 16384, 7), (2, 16385, 256), (3, 50257, 50), (1, 131071, 64),
        (1, 1 << 20, 33), (300, 7, 9), (270, 16, 16), (513, 17, 31), (300, 32, 40), (4100, 40, 5), (4096, 130, 16), (4099, 500, 9), (5000, 300, 3),
-       (66000, 33, 8)]
+       (66000, 33, 8), (65537, 64, 2)]
 
 
 @pytest.mark.parametrize("layout", ["rows", "rows_gap", "classes", "classes_gap"])
