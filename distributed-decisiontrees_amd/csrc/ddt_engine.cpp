@@ -922,15 +922,19 @@ int ddt_host_register(ddt_engine* e, void* ptr, size_t bytes) {
   if (!dg.ok) return fail(e, DDT_EHIP, "hipSetDevice(%d) failed", e->device);
   for (const auto& r : e->pinned)
     if (r.first == ptr) return fail(e, DDT_EINVAL, "ddt_host_register: %p is registered already", ptr);
+  for (const void* p : e->refused)
+    if (p == ptr) return fail(e, DDT_EINVAL, "ddt_host_register: %p is registered already", ptr);
   const hipError_t r = hipHostRegister(ptr, bytes, hipHostRegisterDefault);
-  if (r != hipSuccess) {
-    (void)hipGetLastError();
-    return fail(e, DDT_EHIP, "hipHostRegister(%p, %zu) -> %s", ptr, bytes, hipGetErrorString(r));
-  }
   try {
-    e->pinned.emplace_back(ptr, bytes);
+    if (r == hipSuccess) {
+      e->pinned.emplace_back(ptr, bytes);
+    } else {  // a machine whose driver does not pin memory that exists already: the range keeps going through the feeder's own pinned buffers
+      (void)hipGetLastError();
+      e->refused.push_back(ptr);
+      (void)fail(e, DDT_OK, "hipHostRegister(%p, %zu) -> %s: the range is staged as before", ptr, bytes, hipGetErrorString(r));
+    }
   } catch (const std::bad_alloc&) {
-    (void)hipHostUnregister(ptr);
+    if (r == hipSuccess) (void)hipHostUnregister(ptr);
     return fail(e, DDT_ENOMEM, "ddt_host_register");
   }
   return DDT_OK;
@@ -944,6 +948,11 @@ int ddt_host_unregister(ddt_engine* e, void* ptr) {
       (void)hipDeviceSynchronize();
       (void)hipHostUnregister(ptr);
       e->pinned.erase(e->pinned.begin() + (long)i);
+      return DDT_OK;
+    }
+  for (size_t i = 0; i < e->refused.size(); ++i)
+    if (e->refused[i] == ptr) {
+      e->refused.erase(e->refused.begin() + (long)i);
       return DDT_OK;
     }
   return fail(e, DDT_EINVAL, "ddt_host_unregister: %p was not registered through this engine", ptr);

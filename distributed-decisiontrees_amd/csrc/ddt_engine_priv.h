@@ -122,6 +122,7 @@ struct ddt_engine {
   void* dev_out[ddt::kFeederSlots] = {};
   ddt_copy_pool* pool = nullptr;                         // persistent staging threads (feeder_threads - 1 workers + the caller)
   std::vector<std::pair<void*, size_t>> pinned;          // host ranges the caller pinned through ddt_host_register
+  std::vector<void*> refused;                            // ... and those the driver would not pin: staged like any other
   size_t feeder_cap_rows = 0, feeder_cap_words = 0, feeder_cap_outs = 0;
   // classify workspace (grow-only)
   void* ws = nullptr;

@@ -144,7 +144,8 @@ int ddt_shard_range(uint32_t num_trees, uint32_t shard_index, uint32_t shard_cou
  *    program of the reference hands the FPGA buffers the DMA engine can read; pageable memory has to be staged first).
  *    ddt_host_register pins [ptr, ptr + bytes) for this engine's device (hipHostRegister); ddt_score / ddt_classify calls whose
  *    tuple buffer (and, for ddt_score, score buffer) lies inside a registered range then move the data with the DMA engine
- *    directly -- no staging copy through the engine's own pinned buffers.  Unregister before freeing the memory.          -- */
+ *    directly -- no staging copy through the engine's own pinned buffers.  Where the driver does not pin memory that exists already, the
+ *    range is accepted and staged like any other (ddt_last_error then says so).  Unregister before freeing the memory.     -- */
 int ddt_host_register(ddt_engine* e, void* ptr, size_t bytes);
 int ddt_host_unregister(ddt_engine* e, void* ptr);
 
