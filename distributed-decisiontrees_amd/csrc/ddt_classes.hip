@@ -832,8 +832,16 @@ __global__ __launch_bounds__(top_wave_waves(CM) * 64) void top_wave_kernel(const
           const bool take = x[i] >= bound;
           const uint64_t b = __ballot(take);
           const uint32_t slot = count + lanes_below(b);
-          if (take && slot < kWaveList) list[slot] = candidate(score_key(x[i]), class_of(i));
+          if (take && slot < kWaveList) list[slot] = (uint64_t)__float_as_uint(x[i]) << 32 | class_of(i);
           count += __popcll(b);
+        }
+        if (count <= kWaveList) {  // scores and classes to candidates: once per candidate, not once per place that might hold one
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          __builtin_amdgcn_wave_barrier();
+          for (uint32_t i = lane; i < count; i += 64u) {
+            const uint64_t v = list[i];
+            list[i] = candidate(score_key(__uint_as_float((uint32_t)(v >> 32))), (uint32_t)v);
+          }
         }
       }
       if (count > kWaveList) {  // many wanted, or many that tie: count exactly, bit by bit
