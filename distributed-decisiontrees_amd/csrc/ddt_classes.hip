@@ -295,7 +295,9 @@ struct AdjustTiles {
 };
 
 // Row-major: a tile is `rows` rows times `classes` classes, at most NT * ITER packs of them, ITER per thread.  All loads of a thread --
-// scores, bias, mask, the row's penalties -- are on their way before the history is counted.
+// scores, bias, mask, the row's penalties -- are on their way before the history is counted.  What bounds it with a history is the chain of
+// a tile's latencies (offsets, entries, counters, scores): 64 x 128000 bf16 takes 11 us without histories, 14 with 10 entries a row, 18 with
+// 4096; 32 x 50257 fp32 with 50,000 entries a row 20 us, six rounds of loads for the longest row.
 template <class T, bool HIST, int NT, int ITER>
 __global__ __launch_bounds__(NT) void adjust_rows_kernel(const AdjustArgs a, const AdjustTiles t) {
   constexpr uint32_t N = Pack<T>::N;
@@ -364,7 +366,7 @@ __global__ __launch_bounds__(NT) void adjust_rows_kernel(const AdjustArgs a, con
   }
 }
 
-// class-major: packs run along the rows of one class; a tile's packs per class are a power of two
+// class-major: packs run along the rows of one class; a tile's packs per class are a power of two.  4 M x 10 fp32: 55 us, 5.8 TB/s.
 template <class T, bool HIST>
 __global__ __launch_bounds__(256) void adjust_classes_kernel(const AdjustArgs a, const AdjustTiles t) {
   constexpr uint32_t N = Pack<T>::N;
@@ -515,7 +517,7 @@ __device__ __forceinline__ void write_nothing(const TopArgs& a, uint64_t row, ui
   a.values[row * a.k + rank] = -kInf;
 }
 
-// few classes, few of them wanted: a thread per row, the best k = KK in registers.  Row-major rows are staged in LDS (coalesced loads;
+// few classes, few of them wanted: a thread per row, the best k = KK in registers (4 M x 10 fp32 class-major, k = 3: 52 us for 272 MB, 5.2 TB/s).  Row-major rows are staged in LDS (coalesced loads;
 // the row pitch is an odd number of words), class-major ones are coalesced as they are.
 template <class T>
 __device__ __forceinline__ uint32_t staged_pitch(uint32_t K) {  // elements
@@ -772,7 +774,8 @@ __global__ __launch_bounds__(256) void top_lanes_kernel(const TopArgs a) {
   }
 }
 
-// up to 2048 classes: a wave per row, all its keys in registers (P packs per lane).  Class-major rows are staged through LDS, 16 at a
+// up to 2048 classes: a wave per row, all its scores in registers (P packs per lane).  16384 x 1000 fp32, k = 20: 24 us; the 534 vector
+// instructions per row bound it (14 us' worth of issue), not the 65 MB.  Class-major rows are staged through LDS, 16 at a
 // time for the 8 waves of the block.
 constexpr uint32_t kWaveList = 128;  // candidates that are ranked without an exact count
 __device__ __forceinline__ uint32_t lanes_below(uint64_t ballot) {
@@ -903,7 +906,8 @@ __global__ __launch_bounds__(top_wave_waves(CM) * 64) void top_wave_kernel(const
 // threads' maxima is a bound that at least k scores reach, and only the groups that reach it -- about k of them, 64 packs of
 // 128000 -- are read a second time to list the candidates.  Rows with more candidates than the list holds (scores that tie, or stand
 // in few threads) are narrowed down by counting, bit by bit, over the threads that reach the bound.
-// 512 x 128000 bf16, k = 64: 25 us for the pass (5.2 TB/s), 3 for the bound, 3 for the second look, 2 for the ranks.
+// 512 x 128000 bf16, k = 64: 27 us for 131 MB; with a second look at every pack of the threads that hold candidates -- a cache line each, the
+// whole row over -- it was 41.
 constexpr uint32_t kListCap = 1024, kGroups = 16;
 constexpr uint32_t top_block_words(uint32_t threads) {  // LDS
   return 2u * kListCap + threads + 2u * (threads / 64u) + 4u + threads / 64u + kGroups * threads / 2u;
@@ -1402,7 +1406,8 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void distill_kernel(const Dist
   }
 }
 
-// up to 32 classes: a thread per row, rows staged in LDS and their gradients collected there in fp32.  KK > 0: k = KK entries per row,
+// up to 32 classes: a thread per row, rows staged in LDS and their gradients collected there in fp32.  1 M x 10 fp32, k = 4: 47 us, 1150
+// vector instructions per wave of 64 rows (30 us' worth of issue): the 64-bit numbers of the rows bound it, not the 120 MB.  KK > 0: k = KK entries per row,
 // in registers with their exponentials; KK = 0: any number, read and computed again where they are needed.
 template <class T, int KK, bool GRAD>
 __global__ __launch_bounds__(256) void distill_thread_kernel(const DistillArgs a) {
@@ -1688,8 +1693,9 @@ hipError_t distill_typed(const DistillArgs& a, hipStream_t s) {
   if (packs <= 256u) return distill_rows<T, 64, 4, GRAD>(a, s);
   if (packs <= 512u) return distill_rows<T, 64, 8, GRAD>(a, s);
   // few rows: as many threads on each as there are.  Else enough blocks per CU that one row's ends are hidden behind the other rows'
-  // packs -- for the gradient no more than keep their rows in the 256 MB cache until their second read.  (200 M scores, us, 256 / 512 /
-  // 1024 threads: loss of 50257 fp16-sized classes 89 / 109 / 143; gradient 64000 bf16 253 / 249 / 319, 100000 fp32 516 / 454 / 397.)
+  // packs -- for the gradient no more than keep their rows in the 256 MB cache until their second read, and in registers where a thread's
+  // packs fill them.  (us with 256 / 512 / 1024 threads: loss of 2048 x 50257 fp16 51 / 54 / 72; gradient of 8192 x 128000 bf16
+  // 1123 / 951 / 1148, 2000 x 100000 fp32 457 / 402 / 400; 12200 x 16384 fp32 in registers 336, read twice 372.)
   if (a.n <= 512u) return distill_rows<T, 1024, 0, GRAD>(a, s);
   if (!GRAD) return packs <= 1024u ? distill_rows<T, 256, 4, GRAD>(a, s) : distill_rows<T, 256, 0, GRAD>(a, s);
   if (packs <= 1024u) return distill_rows<T, 256, 4, GRAD>(a, s);
