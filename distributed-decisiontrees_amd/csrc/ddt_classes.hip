@@ -1697,11 +1697,13 @@ hipError_t distill_typed(const DistillArgs& a, hipStream_t s) {
   // packs fill them.  (us with 256 / 512 / 1024 threads: loss of 2048 x 50257 fp16 51 / 54 / 72; gradient of 8192 x 128000 bf16
   // 1123 / 951 / 1148, 2000 x 100000 fp32 457 / 402 / 400; 12200 x 16384 fp32 in registers 336, read twice 372.)
   if (a.n <= 512u) return distill_rows<T, 1024, 0, GRAD>(a, s);
-  if (!GRAD) return packs <= 1024u ? distill_rows<T, 256, 4, GRAD>(a, s) : distill_rows<T, 256, 0, GRAD>(a, s);
   if (packs <= 1024u) return distill_rows<T, 256, 4, GRAD>(a, s);
-  if (packs <= 3072u) return distill_rows<T, 256, 0, GRAD>(a, s);
-  if (packs <= 4096u) return distill_rows<T, 256, 16, GRAD>(a, s);
-  return packs <= 16384u ? distill_rows<T, 512, 0, GRAD>(a, s) : distill_rows<T, 1024, 0, GRAD>(a, s);
+  if constexpr (GRAD) {
+    if (packs <= 3072u) return distill_rows<T, 256, 0, GRAD>(a, s);
+    if (packs <= 4096u) return distill_rows<T, 256, 16, GRAD>(a, s);
+    return packs <= 16384u ? distill_rows<T, 512, 0, GRAD>(a, s) : distill_rows<T, 1024, 0, GRAD>(a, s);
+  }
+  return distill_rows<T, 256, 0, GRAD>(a, s);
 }
 
 }  // namespace
