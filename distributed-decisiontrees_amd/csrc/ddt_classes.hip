@@ -125,13 +125,16 @@ __device__ __forceinline__ uint32_t forgotten(uint32_t v) {
 // x ^ 2: the hardware instruction (1 ulp; results below 2^-126 may come back as 0 -- nothing next to a sum whose largest term is 1)
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// 2^y and ln v beyond fp32 for the rows' own numbers.  2^y: y = n + f with |f| <= 1/2, the power series of e^(f ln 2) to the 8th power in
-// 64 bits (the 9th is below 2e-10 of the sum: a three hundredth of an fp32 rounding), scaled by 2^n: a quarter of the instructions of
-// the library's exp, which aims at the last of the 64 bits.
+// 2^y and ln v beyond fp32 for the rows' own numbers.  2^y: y = n + f with |f| <= 1/2, the power series of e^(f ln 2) to the 10th power in
+// 64 bits (the 11th is below 3e-13 of the sum; a loss is a difference of such logarithms, and where a student has learned its teacher
+// one of 1e-4 is left of terms near 10: 3e-8 of it), scaled by 2^n: a third of the instructions of the library's exp, which aims at the
+// last of the 64 bits.
 __device__ __forceinline__ double exp2_64(double y) {
   y = y < -1100.0 ? -1100.0 : y > 1100.0 ? 1100.0 : y;  // (NaN stays)
   const double n = __builtin_rint(y), f = (y - n) * 0.69314718055994530942;
-  double p = 1.0 / 40320.0;
+  double p = 1.0 / 3628800.0;
+  p = fma(p, f, 1.0 / 362880.0);
+  p = fma(p, f, 1.0 / 40320.0);
   p = fma(p, f, 1.0 / 5040.0);
   p = fma(p, f, 1.0 / 720.0);
   p = fma(p, f, 1.0 / 120.0);
