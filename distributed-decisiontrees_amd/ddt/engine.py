@@ -277,20 +277,27 @@ class Engine:
             raise ValueError(f"{what}: {t.dtype}, must be one of {list(_torch_types().codes)}")
         if t.dim() != 2:
             raise ValueError(f"{what}: {t.dim()} dimensions, must be 2")
-        p, shape, stride = self._tensor(t, what, t.dtype), t.shape, t.stride()
-        return _lib.Scores(p, shape[rows], stride[rows], stride[1 - rows], shape[1 - rows], code)
+        if not t.is_cuda or t.get_device() != self.device:
+            raise ValueError(f"{what}: on {t.device}, the engine is on cuda:{self.device}")
+        a, b = t.shape
+        c, d = t.stride()
+        return _lib.Scores(t.data_ptr(), b, d, c, a, code) if rows else _lib.Scores(t.data_ptr(), a, c, d, b, code)
 
     def _stream(self, stream):
         """handle of the stream of a call"""
         return _torch_types().raw_stream(self.device) if stream is None else stream.cuda_stream
 
     @staticmethod
-    def _empty(like, shape, dtype, stream, strides=None):
-        """uninitialised tensor on the device of `like`, allocated on the stream of the call"""
-        if stream is not None:
+    def _allocator(like, stream):
+        """like.new_empty on the stream of the call"""
+        if stream is None:
+            return like.new_empty
+
+        def on_stream(*args, **kw):
             with _torch_types().torch.cuda.stream(stream):
-                return Engine._empty(like, shape, dtype, None, strides)
-        return like.new_empty(shape, dtype=dtype) if strides is None else like.new_empty_strided(shape, strides)
+                return like.new_empty(*args, **kw)
+
+        return on_stream
 
     def adjust_device(self, class_scores, bias=None, allowed=None, history=None, history_first=None, history_prompt=None,
                       repetition=None, frequency=None, presence=None, out=None, stream=None):
@@ -342,8 +349,11 @@ class Engine:
             raise ValueError("history_first, history_prompt and penalties need a history")
         if out is None:
             row_major = s.class_stride == 1 and (s.row_stride >= K or n <= 1)
-            out = self._empty(class_scores, (K, n), None, stream, (1, K) if row_major else (n, 1))
-        o = self._scores(out, "out")
+            new = self._allocator(class_scores, stream)
+            out = new((n, K)).t() if row_major else new((K, n))
+            o = _lib.Scores(out.data_ptr(), n, K if row_major else 1, 1 if row_major else n, K, s.dtype)
+        else:
+            o = self._scores(out, "out")
         self._check(self._L.ddt_adjust_scores_device(self._h, C.byref(s), C.byref(a), C.byref(o), self._stream(stream)))
         return out
 
@@ -355,12 +365,23 @@ class Engine:
         T = _torch_types()
         s = self._scores(class_scores, "class_scores")
         n = s.rows
-        ids = self._empty(class_scores, (n, k), T.i32, stream) if ids is None else ids
-        values = self._empty(class_scores, (n, k), T.f32, stream) if values is None else values
-        lse = self._empty(class_scores, (n,), T.f32, stream) if lse is None else lse
-        self._check(self._L.ddt_top_scores_device(
-            self._h, C.byref(s), k, temperature, self._packed(ids, "ids", T.i32, (n, k)),
-            self._packed(values, "values", T.f32, (n, k)), self._packed(lse, "lse", T.f32, (n,)), self._stream(stream)))
+        new = self._allocator(class_scores, stream)
+        if ids is None:
+            ids = new((n, k), dtype=T.i32)
+            p_ids = ids.data_ptr()
+        else:
+            p_ids = self._packed(ids, "ids", T.i32, (n, k))
+        if values is None:
+            values = new((n, k), dtype=T.f32)
+            p_values = values.data_ptr()
+        else:
+            p_values = self._packed(values, "values", T.f32, (n, k))
+        if lse is None:
+            lse = new((n,), dtype=T.f32)
+            p_lse = lse.data_ptr()
+        else:
+            p_lse = self._packed(lse, "lse", T.f32, (n,))
+        self._check(self._L.ddt_top_scores_device(self._h, C.byref(s), k, temperature, p_ids, p_values, p_lse, self._stream(stream)))
         return ids, values, lse
 
     def top_classes_device(self, d_tuples, k: int, temperature: float = 1.0, stream=None, **adjust):
@@ -393,9 +414,12 @@ class Engine:
         T = _torch_types()
         s = self._scores(student, "student", rows=0)
         t = self._teacher(s.rows, ids, values, lse, temperature)
-        loss = self._empty(student, (s.rows,), T.f32, stream) if loss is None else loss
-        self._check(self._L.ddt_distill_device(self._h, C.byref(s), C.byref(t), self._packed(loss, "loss", T.f32, (s.rows,)),
-                                               self._stream(stream)))
+        if loss is None:
+            loss = self._allocator(student, stream)((s.rows,), dtype=T.f32)
+            p_loss = loss.data_ptr()
+        else:
+            p_loss = self._packed(loss, "loss", T.f32, (s.rows,))
+        self._check(self._L.ddt_distill_device(self._h, C.byref(s), C.byref(t), p_loss, self._stream(stream)))
         return loss
 
     def distill_grad_device(self, student, ids, values, lse=None, row_weight=None, temperature: float = 1.0, loss=None, grad=None,
@@ -410,11 +434,18 @@ class Engine:
         w, w_stride = None, 0
         if row_weight is not None:
             w, w_stride = self._tensor(row_weight, "row_weight", T.f32, (n,)), row_weight.stride(0) if n > 1 else 0
-        loss = self._empty(student, (n,), T.f32, stream) if loss is None else loss
-        grad = self._empty(student, (n, s.num_classes), student.dtype, stream) if grad is None else grad
-        g = self._scores(grad, "grad", rows=0)
-        self._check(self._L.ddt_distill_grad_device(self._h, C.byref(s), C.byref(t), w, w_stride,
-                                                    self._packed(loss, "loss", T.f32, (n,)), C.byref(g), self._stream(stream)))
+        new = self._allocator(student, stream)
+        if loss is None:
+            loss = new((n,), dtype=T.f32)
+            p_loss = loss.data_ptr()
+        else:
+            p_loss = self._packed(loss, "loss", T.f32, (n,))
+        if grad is None:
+            grad = new((n, s.num_classes))
+            g = _lib.Scores(grad.data_ptr(), n, s.num_classes, 1, s.num_classes, s.dtype)
+        else:
+            g = self._scores(grad, "grad", rows=0)
+        self._check(self._L.ddt_distill_grad_device(self._h, C.byref(s), C.byref(t), w, w_stride, p_loss, C.byref(g), self._stream(stream)))
         return loss, grad
 
     def distill(self, student, ids, values, lse=None, temperature: float = 1.0):
