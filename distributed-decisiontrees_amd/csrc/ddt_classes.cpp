@@ -87,7 +87,8 @@ int distill(ddt_engine* e, const ddt_scores_t* s, const ddt_teacher_t* t, const 
   if (!dg.ok) return fail(e, DDT_EHIP, "hipSetDevice(%d) failed", e->device);
   DistillArgs a{};
   a.in = s->data, a.n = s->rows, a.stride = l.stride, a.K = s->num_classes, a.k = t->k;
-  a.ids = t->ids, a.values = t->values, a.teacher_stride = t->row_stride, a.lse = t->lse, a.temperature = t->temperature;
+  a.ids = t->ids, a.values = t->values, a.teacher_stride = t->row_stride, a.lse = t->lse;
+  a.inv_T = 1.0 / t->temperature, a.scale = (float)(kLog2e / t->temperature);
   a.loss = d_loss;
   if (want_grad) a.weight = weight, a.weight_stride = weight_stride, a.grad = grad->data, a.grad_stride = lg.stride;
   return run(e, "distill", launch_distill(a, s->dtype, reinterpret_cast<hipStream_t>(stream)));
@@ -153,7 +154,8 @@ int ddt_top_scores_device(ddt_engine* e, const ddt_scores_t* s, uint32_t k, doub
   DeviceGuard dg(e->device);
   if (!dg.ok) return fail(e, DDT_EHIP, "hipSetDevice(%d) failed", e->device);
   TopArgs a{};
-  a.in = s->data, a.n = s->rows, a.stride = l.stride, a.K = s->num_classes, a.k = k, a.temperature = temperature;
+  a.in = s->data, a.n = s->rows, a.stride = l.stride, a.K = s->num_classes, a.k = k;
+  a.inv_T = 1.0 / temperature, a.scale = (float)(kLog2e / temperature);
   a.ids = d_ids, a.values = d_values, a.lse = d_lse;
   return run(e, "top", launch_top(a, s->dtype, l.class_major, reinterpret_cast<hipStream_t>(stream)));
 }

@@ -6,6 +6,8 @@
 
 namespace ddt {
 
+constexpr double kLog2e = 1.4426950408889634;
+
 struct AdjustArgs {
   const void* in;
   void* out;
@@ -26,7 +28,8 @@ struct TopArgs {
   const void* in;
   uint64_t n, stride;
   uint32_t K, k;
-  double temperature;
+  double inv_T;  // 1 / temperature
+  float scale;   // log2(e) / temperature
   int32_t* ids;
   float* values;
   float* lse;  // may be NULL
@@ -40,7 +43,8 @@ struct DistillArgs {
   const float* values;
   uint64_t teacher_stride;
   const float* lse;  // NULL: the teacher's mass is on the listed classes
-  double temperature;
+  double inv_T;  // 1 / temperature
+  float scale;   // log2(e) / temperature
   const float* weight;  // NULL = 1; only with a gradient
   uint64_t weight_stride;
   float* loss;  // may be NULL with a gradient

@@ -18,7 +18,6 @@ namespace {
 extern __shared__ uint32_t lds_words[];
 
 constexpr float kInf = __builtin_inff();
-constexpr double kLog2e = 1.4426950408889634;
 
 template <class T>
 struct Pack {
@@ -151,6 +150,13 @@ __device__ __forceinline__ double log_64(double v) {
   if (v == 0.0) return -__builtin_inf();
   const double y = (double)__builtin_amdgcn_logf((float)v), r = fma(v, exp2_64(-y), -1.0);
   return fma(y, 0.69314718055994530942, r - 0.5 * r * r);
+}
+
+// 1 / v for sums relative to their largest term: the hardware's first digits and two Newton steps
+__device__ __forceinline__ double inverse_64(double v) {
+  double r = __builtin_amdgcn_rcp(v);
+  r = fma(fma(-v, r, 1.0), r, r);
+  return fma(fma(-v, r, 1.0), r, r);
 }
 
 // reductions over a wave: five moves within rows of 16 lanes and across them (DPP: no LDS), the last lane then holds the result of all
@@ -557,7 +563,7 @@ template <class T, bool CM, int KK>
 __global__ __launch_bounds__(256) void top_thread_kernel(const TopArgs a) {
   T* stage = reinterpret_cast<T*>(lds_words);
   const uint32_t pitch = staged_pitch<T>(a.K);
-  const float c2 = (float)(kLog2e / a.temperature);
+  const float c2 = a.scale;
   const uint64_t step = (uint64_t)gridDim.x * 256u;
   for (uint64_t r0 = (uint64_t)blockIdx.x * 256u; r0 < a.n; r0 += step) {
     const uint32_t rows = (uint32_t)(a.n - r0 < 256u ? a.n - r0 : 256u);
@@ -603,7 +609,7 @@ __global__ __launch_bounds__(256) void top_thread_kernel(const TopArgs a) {
     }
     __builtin_memcpy(a.ids + row * KK, id, sizeof(id));  // (one store: a wave writes one piece)
     __builtin_memcpy(a.values + row * KK, v, sizeof(v));
-    if (a.lse) a.lse[row] = log_sum(e, 1.0 / a.temperature);
+    if (a.lse) a.lse[row] = log_sum(e, a.inv_T);
   }
 }
 
@@ -642,7 +648,7 @@ __global__ __launch_bounds__(256) void top_rank_kernel(const TopArgs a) {
   const uint32_t pitch = staged_pitch<T>(a.K), columns = a.k < a.K ? a.k : a.K, opitch = columns | 1u;
   float* out_value = reinterpret_cast<float*>(lds_words);  // (takes the place of the staged rows, which are in registers by then)
   int32_t* out_id = reinterpret_cast<int32_t*>(lds_words + 256u * opitch);
-  const float c2 = (float)(kLog2e / a.temperature);
+  const float c2 = a.scale;
   for (uint64_t r0 = (uint64_t)blockIdx.x * 256u; r0 < a.n; r0 += (uint64_t)gridDim.x * 256u) {
     const uint32_t rows = (uint32_t)(a.n - r0 < 256u ? a.n - r0 : 256u), tid = forgotten(threadIdx.x);
     const T* in = static_cast<const T*>(a.in);
@@ -667,7 +673,7 @@ __global__ __launch_bounds__(256) void top_rank_kernel(const TopArgs a) {
         e.s += exp2_fast((x[c] - e.m) * c2);
         x[c] = x[c] > -kInf ? x[c] : -kInf;  // (NaN is no candidate)
       }
-      if (a.lse) a.lse[r0 + tid] = log_sum(e, 1.0 / a.temperature);
+      if (a.lse) a.lse[r0 + tid] = log_sum(e, a.inv_T);
       uint32_t rank[KP];
 #pragma unroll
       for (int c = 0; c < KP; ++c) rank[c] = c;
@@ -715,7 +721,7 @@ template <class T, bool CM, int P>
 __global__ __launch_bounds__(256) void top_lanes_kernel(const TopArgs a) {
   constexpr int N = (int)Pack<T>::N, E = P * N;
   float* stage = reinterpret_cast<float*>(lds_words);
-  const float c2 = (float)(kLog2e / a.temperature);
+  const float c2 = a.scale;
   for (uint64_t r0 = (uint64_t)blockIdx.x * 16u; r0 < a.n; r0 += (uint64_t)gridDim.x * 16u) {
     if (CM) {
       __syncthreads();
@@ -746,7 +752,7 @@ __global__ __launch_bounds__(256) void top_lanes_kernel(const TopArgs a) {
 #pragma unroll
     for (int i = 0; i < E; ++i) e.s += exp2_fast((x[i] - e.m) * c2);
     e.s = lanes_sum<16>(e.s);
-    if (a.lse && lane == 0u) a.lse[row] = log_sum(e, 1.0 / a.temperature);
+    if (a.lse && lane == 0u) a.lse[row] = log_sum(e, a.inv_T);
     float value = -kInf;
     int32_t id = -1;
     for (uint32_t j = 0; j < a.k; ++j) {
@@ -794,7 +800,7 @@ __global__ __launch_bounds__(top_wave_waves(CM) * 64) void top_wave_kernel(const
   const uint32_t wave = threadIdx.x >> 6;
   uint64_t* list = reinterpret_cast<uint64_t*>(lds_words) + wave * wave_list(a.k);  // the wave's selected candidates
   float* stage = reinterpret_cast<float*>(reinterpret_cast<uint64_t*>(lds_words) + kWaves * wave_list(a.k));  // class-major
-  const float c2 = (float)(kLog2e / a.temperature);
+  const float c2 = a.scale;
   for (uint64_t r0 = (uint64_t)blockIdx.x * kRows; r0 < a.n; r0 += (uint64_t)gridDim.x * kRows) {
     if (CM) {
       __syncthreads();
@@ -824,7 +830,7 @@ __global__ __launch_bounds__(top_wave_waves(CM) * 64) void top_wave_kernel(const
 #pragma unroll
       for (int i = 0; i < E; ++i) e.s += exp2_fast((x[i] - e.m) * c2);
       e.s = wave_sum(e.s);
-      if (a.lse && lane == 0u) a.lse[row] = log_sum(e, 1.0 / a.temperature);
+      if (a.lse && lane == 0u) a.lse[row] = log_sum(e, a.inv_T);
       // A bound that at least k scores reach: the k-th largest of the lanes' best, or a little below it.  What reaches it is listed and
       // ranked.
       uint32_t count = kWaveList + 1u;
@@ -929,7 +935,7 @@ __global__ __launch_bounds__(NT) void top_block_kernel(const TopArgs a) {
   uint16_t* group_max = reinterpret_cast<uint16_t*>(ctl + 4 + kWaves);  // [kGroups][NT]
   const uint32_t packs = (a.K + N - 1u) / N, chunks = (packs + 4u * NT - 1u) / (4u * NT);
   const uint32_t per_group = (chunks + kGroups - 1u) / kGroups;  // chunks
-  const float c2 = (float)(kLog2e / a.temperature);
+  const float c2 = a.scale;
   for (uint64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
     const T* in = static_cast<const T*>(a.in) + row * a.stride;
     const uint32_t tid = forgotten(threadIdx.x), lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -1001,7 +1007,7 @@ __global__ __launch_bounds__(NT) void top_block_kernel(const TopArgs a) {
       ExpSum w;
       w.m = lane < kWaves ? part[2 * lane] : -FLT_MAX, w.s = lane < kWaves ? part[2 * lane + 1] : 0.f;
       w.reduce_wave(c2);
-      if (lane == 0u) a.lse[row] = log_sum(w, 1.0 / a.temperature);
+      if (lane == 0u) a.lse[row] = log_sum(w, a.inv_T);
     }
     __syncthreads();
     const uint32_t bound = ctl[0];
@@ -1143,7 +1149,7 @@ struct Entries {
 template <class T, int L, bool GRAD>
 __device__ __forceinline__ RowGrad row_loss(const DistillArgs& a, uint64_t row, const Entries& en, uint32_t lane, const ExpSum& o) {
   // the student's scale is the fp32 one of the sums outside S, for all its classes: p stays a softmax, of a temperature off by 2^-25
-  const double inv_T = 1.0 / a.temperature, x_scale = (double)(float)(kLog2e / a.temperature);
+  const double inv_T = a.inv_T, x_scale = (double)a.scale;
   constexpr double kLn2 = 0.69314718055994530942;
   float xm = -FLT_MAX, tm = -FLT_MAX;
   for (uint32_t j = lane; j < a.k; j += L)
@@ -1162,15 +1168,15 @@ __device__ __forceinline__ RowGrad row_loss(const DistillArgs& a, uint64_t row, 
   zs = lanes_sum<L>(zs), ts = lanes_sum<L>(ts);
   const double far = exp2_64(((double)o.m - (double)M) * x_scale), Z = (double)o.s * far + zs, log_Z = log_64(Z);
   // without lse the q are still to be divided by their sum
-  const double log_T = a.lse ? shift : shift + log_64(ts), scale = a.lse ? 1.0 : 1.0 / ts;
-  double Q = a.lse ? ts : 1.0, rest = 0.0, loss = 0.0;
+  const double log_T = a.lse ? shift : shift + log_64(ts), scale = a.lse ? 1.0 : inverse_64(ts);
+  double Q = a.lse ? ts : 1.0, rest_s = 0.0, loss = 0.0;  // rest_s = q_R / s_o
   for (uint32_t j = lane; j < a.k; j += L)
     if (en.id[j] >= 0 && !(en.q[j] == 0.0))
       loss += en.q[j] * scale * (((double)en.t[j] * inv_T - log_T) - (((double)en.x[j] - (double)M) * x_scale * kLn2 - log_Z));
   loss = lanes_sum<L>(loss);
   if (a.lse && o.s > 0.f && Q < 1.0) {
-    rest = 1.0 - Q;
-    loss += rest * (log_64(rest) - (((double)o.m - (double)M) * x_scale * kLn2 + log_64((double)o.s) - log_Z));
+    rest_s = (1.0 - Q) * inverse_64((double)o.s);
+    loss += (1.0 - Q) * (log_64(rest_s) - (((double)o.m - (double)M) * x_scale * kLn2 - log_Z));
     Q = 1.0;
   }
   if (a.loss && lane == 0u) a.loss[row] = (float)loss;
@@ -1178,7 +1184,8 @@ __device__ __forceinline__ RowGrad row_loss(const DistillArgs& a, uint64_t row, 
   if (GRAD) {
     const double w = (a.weight ? (double)a.weight[row * a.weight_stride] : 1.0) * inv_T;
     // (nothing outside S: no gradient there; nothing in the whole row: NaN, as its softmax)
-    g.coef = !(o.s == 0.f) ? (float)((Q * far / Z - rest / (double)o.s) * w) : Z == 0.0 ? __builtin_nanf("") : 0.f;
+    const double p_scale = Q * inverse_64(Z);
+    g.coef = !(o.s == 0.f) ? (float)((p_scale * far - rest_s) * w) : Z == 0.0 ? __builtin_nanf("") : 0.f;
     T* out = static_cast<T*>(a.grad) + row * a.grad_stride;
     for (uint32_t j = lane; j < a.k; j += L) {
       const int32_t id = en.id[j];
@@ -1186,7 +1193,7 @@ __device__ __forceinline__ RowGrad row_loss(const DistillArgs& a, uint64_t row, 
       double qc = en.q[j];
       for (uint32_t i = j + 1u; i < a.k; ++i)  // further entries of this class, in their order
         if (en.id[i] == (id | kAgain)) qc += en.q[i];
-      out[id] = (T)(float)((en.e[j] / Z * Q - qc * scale) * w);
+      out[id] = (T)(float)((en.e[j] * p_scale - qc * scale) * w);
     }
   }
   return g;
@@ -1211,7 +1218,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void distill_kernel(const Dist
   float* part = reinterpret_cast<float*>(ctl + 4);       // [2 * kWaves]
   uint32_t* bitmap = ctl + 4 + 2u * kWaves;              // [words]
   const uint32_t packs = (a.K + N - 1u) / N;
-  const float c2 = (float)(kLog2e / a.temperature);
+  const float c2 = a.scale;
   auto sync = [] {
     if (NT <= 64) {
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -1418,8 +1425,8 @@ __global__ __launch_bounds__(256) void distill_thread_kernel(const DistillArgs a
   const uint32_t pitch = staged_pitch<T>(a.K), gpitch = a.K | 1u;
   float* gstage = reinterpret_cast<float*>(lds_words + (256u * pitch * sizeof(T)) / 4u);
   constexpr double kLn2 = 0.69314718055994530942;
-  const float c2 = (float)(kLog2e / a.temperature);
-  const double inv_T = 1.0 / a.temperature, x_scale = (double)c2;
+  const float c2 = a.scale;
+  const double inv_T = a.inv_T, x_scale = (double)c2;
   for (uint64_t r0 = (uint64_t)blockIdx.x * 256u; r0 < a.n; r0 += (uint64_t)gridDim.x * 256u) {
     const uint32_t rows = (uint32_t)(a.n - r0 < 256u ? a.n - r0 : 256u);
     const uint32_t tid = forgotten(threadIdx.x);
@@ -1487,17 +1494,17 @@ __global__ __launch_bounds__(256) void distill_thread_kernel(const DistillArgs a
           open &= ~(1u << c);
         });
         const double far = exp2_64(((double)om - (double)M) * x_scale), Z = (double)os * far + zs, log_Z = log_64(Z);
-        const double log_T = a.lse ? shift : shift + log_64(ts), scale = a.lse ? 1.0 : 1.0 / ts;
-        double Q = a.lse ? ts : 1.0, rest = 0.0, loss = 0.0;
+        const double log_T = a.lse ? shift : shift + log_64(ts), scale = a.lse ? 1.0 : inverse_64(ts);
+        double Q = a.lse ? ts : 1.0, rest_s = 0.0, loss = 0.0;
         if (a.lse && os > 0.f && Q < 1.0) {
-          rest = 1.0 - Q;
-          loss = rest * (log_64(rest) - (((double)om - (double)M) * x_scale * kLn2 + log_64((double)os) - log_Z));
+          rest_s = (1.0 - Q) * inverse_64((double)os);
+          loss = (1.0 - Q) * (log_64(rest_s) - (((double)om - (double)M) * x_scale * kLn2 - log_Z));
           Q = 1.0;
         }
-        const double w = (double)weight * inv_T, p_scale = Q / Z;
+        const double w = (double)weight * inv_T, p_scale = Q * inverse_64(Z);
         if (GRAD) {
           // (nothing outside the list: no gradient there; nothing in the whole row: NaN, as its softmax)
-          const float coef = !(os == 0.f) ? (float)((p_scale * far - rest / (double)os) * w) : Z == 0.0 ? __builtin_nanf("") : 0.f;
+          const float coef = !(os == 0.f) ? (float)((p_scale * far - rest_s) * w) : Z == 0.0 ? __builtin_nanf("") : 0.f;
 #pragma unroll 4
           for (uint32_t c = 0; c < a.K; ++c) g[c] *= coef;
         }
@@ -1702,7 +1709,7 @@ hipError_t distill_typed(const DistillArgs& a, hipStream_t s) {
   if (a.n <= 512u) return distill_rows<T, 1024, 0, GRAD>(a, s);
   if (packs <= 1024u) return distill_rows<T, 256, 4, GRAD>(a, s);
   if constexpr (GRAD) {
-    if (packs <= 3072u) return distill_rows<T, 256, 0, GRAD>(a, s);
+    if (packs <= 3000u) return distill_rows<T, 256, 0, GRAD>(a, s);
     if (packs <= 4096u) return distill_rows<T, 256, 16, GRAD>(a, s);
     return packs <= 16384u ? distill_rows<T, 512, 0, GRAD>(a, s) : distill_rows<T, 1024, 0, GRAD>(a, s);
   }
