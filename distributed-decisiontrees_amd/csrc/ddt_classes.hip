@@ -1169,7 +1169,7 @@ __device__ __forceinline__ RowGrad row_loss(const DistillArgs& a, uint64_t row, 
   const double far = exp2_64(((double)o.m - (double)M) * x_scale), Z = (double)o.s * far + zs, log_Z = log_64(Z);
   // without lse the q are still to be divided by their sum
   const double log_T = a.lse ? shift : shift + log_64(ts), scale = a.lse ? 1.0 : inverse_64(ts);
-  double Q = a.lse ? ts : 1.0, rest_s = 0.0, loss = 0.0;  // rest_s = q_R / s_o
+  double Q = a.lse ? ts : ts * scale, rest_s = 0.0, loss = 0.0;  // (1 without lse, or NaN); rest_s = q_R / s_o
   for (uint32_t j = lane; j < a.k; j += L)
     if (en.id[j] >= 0 && !(en.q[j] == 0.0))
       loss += en.q[j] * scale * (((double)en.t[j] * inv_T - log_T) - (((double)en.x[j] - (double)M) * x_scale * kLn2 - log_Z));
@@ -1179,13 +1179,14 @@ __device__ __forceinline__ RowGrad row_loss(const DistillArgs& a, uint64_t row, 
     loss += (1.0 - Q) * (log_64(rest_s) - (((double)o.m - (double)M) * x_scale * kLn2 - log_Z));
     Q = 1.0;
   }
-  if (a.loss && lane == 0u) a.loss[row] = (float)loss;
+  // a student's row without a softmax (NaN, +inf, or nothing but -inf), or a teacher's: also where no entry's probability carries it on
+  const bool none = !(Z > 0.0 && Q >= 0.0 && Q < __builtin_inf());
+  if (a.loss && lane == 0u) a.loss[row] = none ? __builtin_nanf("") : (float)loss;
   RowGrad g = {o.m, 0.f};
   if (GRAD) {
     const double w = (a.weight ? (double)a.weight[row * a.weight_stride] : 1.0) * inv_T;
-    // (nothing outside S: no gradient there; nothing in the whole row: NaN, as its softmax)
-    const double p_scale = Q * inverse_64(Z);
-    g.coef = !(o.s == 0.f) ? (float)((p_scale * far - rest_s) * w) : Z == 0.0 ? __builtin_nanf("") : 0.f;
+    const double p_scale = none ? __builtin_nan("") : Q * inverse_64(Z);
+    g.coef = o.s == 0.f && !none ? 0.f : (float)((p_scale * far - rest_s) * w);  // (nothing outside S: no gradient there)
     T* out = static_cast<T*>(a.grad) + row * a.grad_stride;
     for (uint32_t j = lane; j < a.k; j += L) {
       const int32_t id = en.id[j];
@@ -1495,16 +1496,16 @@ __global__ __launch_bounds__(256) void distill_thread_kernel(const DistillArgs a
         });
         const double far = exp2_64(((double)om - (double)M) * x_scale), Z = (double)os * far + zs, log_Z = log_64(Z);
         const double log_T = a.lse ? shift : shift + log_64(ts), scale = a.lse ? 1.0 : inverse_64(ts);
-        double Q = a.lse ? ts : 1.0, rest_s = 0.0, loss = 0.0;
+        double Q = a.lse ? ts : ts * scale, rest_s = 0.0, loss = 0.0;
         if (a.lse && os > 0.f && Q < 1.0) {
           rest_s = (1.0 - Q) * inverse_64((double)os);
           loss = (1.0 - Q) * (log_64(rest_s) - (((double)om - (double)M) * x_scale * kLn2 - log_Z));
           Q = 1.0;
         }
-        const double w = (double)weight * inv_T, p_scale = Q * inverse_64(Z);
+        const bool none = !(Z > 0.0 && Q >= 0.0 && Q < __builtin_inf());  // (as in row_loss)
+        const double w = (double)weight * inv_T, p_scale = none ? __builtin_nan("") : Q * inverse_64(Z);
         if (GRAD) {
-          // (nothing outside the list: no gradient there; nothing in the whole row: NaN, as its softmax)
-          const float coef = !(os == 0.f) ? (float)((p_scale * far - rest_s) * w) : Z == 0.0 ? __builtin_nanf("") : 0.f;
+          const float coef = os == 0.f && !none ? 0.f : (float)((p_scale * far - rest_s) * w);
 #pragma unroll 4
           for (uint32_t c = 0; c < a.K; ++c) g[c] *= coef;
         }
@@ -1522,7 +1523,7 @@ __global__ __launch_bounds__(256) void distill_thread_kernel(const DistillArgs a
             g[c] = (float)(((KK > 0 ? eq[KK > 0 ? j : 0][0] : exp2_64(student(c))) * p_scale - qc * scale) * w);
           }
         });
-        if (a.loss) a.loss[row] = (float)loss;
+        if (a.loss) a.loss[row] = none ? __builtin_nanf("") : (float)loss;
       }
     }
     if (GRAD) {

@@ -219,7 +219,8 @@ typedef struct ddt_adjust_t {
   uint64_t        bias_row_stride, bias_class_stride;
   const uint32_t* allowed;            /* class c is allowed in row r: bit c % 32 of allowed[r * allowed_row_stride + c / 32]               */
   uint64_t        allowed_row_stride; /* words; 0 = one mask for every row, else >= ceil(num_classes / 32)                                */
-  const int32_t*  history;            /* classes, history_len of them; a number outside 0 .. num_classes - 1 stands for no class           */
+  const int32_t*  history;            /* classes, history_len of them; a number outside 0 .. num_classes - 1 stands for no class.
+                                         A row holds a class fewer than 2^31 times                                                       */
   const int64_t*  history_first;      /* [rows + 1]: row r's history is [history_first[r], history_first[r + 1]), clamped to the array      */
   uint64_t        history_len;
   const int32_t*  history_prompt;     /* [rows]: that many entries at the front of the row's history are its prompt part                   */
@@ -250,7 +251,8 @@ typedef struct ddt_teacher_t {
 /* Distillation loss of a student's scores (row-major), p = softmax(student / T):
  *      loss[r] = sum_j q_j (log q_j - log p_(id j)) + q_R (log q_R - log p_R),   p_R = the student's probability of the classes not listed
  * The rest is left out where q_R or p_R is 0.  A row without entries: 0.  A class listed twice counts with both entries.  A row of the
- * student that holds NaN or +inf, or nothing but -inf, has no softmax: its loss and gradient are NaN.
+ * student that holds NaN or +inf, or nothing but -inf, has no softmax: its loss and gradient are NaN.  So are those of a row whose teacher
+ * has none (NaN or +inf among its entries; without lse nothing but -inf).
  * ..._grad: also grad (row-major, the student's type; may be the student's own buffer) =
  *      row_weight[r] d loss[r] / d student[r][c] = row_weight[r] / T (p_c Q - sum of q_j with id c - [c not listed] q_R p_c / p_R),
  *      Q = sum q_j + q_R; row_weight[r * row_weight_stride] (stride 0 = one for all; NULL = 1) is the gradient that arrives at loss[r].

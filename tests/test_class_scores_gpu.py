@@ -465,6 +465,38 @@ def test_distill_students_with_masked_classes(engine, n, K, rest):
     assert loss[2] == math.inf and loss[7] == 0 and not grad[7].any() and loss[3].isnan() and grad[3].isnan().all()
 
 
+@pytest.mark.parametrize("n,K,k", [(12, 10, 3), (12, 20, 7), (4100, 60, 5), (12, 500, 9), (600, 5003, 4), (600, 40001, 4), (12, 50257, 4)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_distill_rows_without_a_softmax(engine, n, K, k, dtype):
+    """NaN, wherever the row has no softmax of its student's or its teacher's -- also where all listed probabilities are 0; ordinary rows
+    next to them stay as they are"""
+    x = matrix(n, K, dtype, seed=5).t().contiguous()
+    ids, vals, lse = teacher_of(n, K, k, 2.0, ragged=False)
+    outside = [int(np.setdiff1d(np.arange(k + 1), ids[r])[0]) for r in range(n)]
+    dev = lambda a: torch.from_numpy(a).cuda()
+    plain, plain_grad = engine.distill_grad_device(x, dev(ids), dev(vals), dev(lse), temperature=2.0)
+    want, grad, size = distill64(x.double().cpu().numpy(), ids, vals, lse, 2.0, np.ones(n))
+    close(plain.double().cpu(), want, 200 * U + U * np.abs(want))
+    fi = torch.finfo(x.dtype)
+    close(plain_grad.double().cpu(), grad, size + (fi.eps / 2) * (np.abs(grad) + size) + fi.smallest_normal * fi.eps / 2 + 2.0 ** -126)
+    vals[:4] = -np.inf                                # rows 0 .. 3: every listed probability is 0, the rest's is 1
+    x[0, outside[0]], x[1, outside[1]], x[2] = float("nan"), float("inf"), float("-inf")
+    vals[4, k - 1], vals[5, 0], lse[6] = np.nan, np.inf, np.nan
+    x[7, int(ids[7, 0])] = float("nan")
+    for given, bad, zero_rest in ((dev(lse), [0, 1, 2, 4, 5, 6, 7], [3]), (None, [0, 1, 2, 3, 4, 5, 7], [])):
+        loss, grad = engine.distill_grad_device(x, dev(ids), dev(vals), given, temperature=2.0)
+        assert torch.equal(engine.distill_device(x, dev(ids), dev(vals), given, temperature=2.0).isnan(), loss.isnan())
+        assert loss.isnan().nonzero().flatten().tolist() == bad
+        assert grad[bad].isnan().all() and not grad.isnan()[[r for r in range(n) if r not in bad]].any()
+        if given is not None:
+            assert torch.equal(loss[8:], plain[8:]) and torch.equal(grad[8:], plain_grad[8:])
+        for r in zero_rest:                           # loss = -log p_R
+            z = x[r].double().cpu().numpy() / 2.0
+            e = np.exp(z - z.max())
+            log_p = np.log(np.delete(e, ids[r]).sum() / e.sum())
+            close(loss[r].item(), -log_p, 200 * U + U * abs(log_p))
+
+
 @pytest.mark.parametrize("n,K", [(5, 10), (5, 500), (5, 5000), (5, 50257), (4100, 100), (4100, 1000), (600, 9000), (600, 33000), (520, 150001)])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_distill_gradient_in_place(engine, n, K, dtype):
