@@ -285,7 +285,11 @@ class Engine:
 
     def _stream(self, stream):
         """handle of the stream of a call"""
-        return _torch_types().raw_stream(self.device) if stream is None else stream.cuda_stream
+        if stream is None:
+            return _torch_types().raw_stream(self.device)
+        if stream.device_index != self.device:
+            raise ValueError(f"stream: of cuda:{stream.device_index}, the engine is on cuda:{self.device}")
+        return stream.cuda_stream
 
     @staticmethod
     def _allocator(like, stream):
@@ -403,7 +407,7 @@ class Engine:
         k = ids.shape[-1] if ids.dim() else 0
         p, v = self._tensor(ids, "ids", T.i32, (n, k)), self._tensor(values, "values", T.f32, (n, k))
         by_row, by_entry = ids.stride()
-        if ids.stride() != values.stride() and n > 1 or k > 1 and (by_entry != 1 or values.stride(1) != 1):
+        if n > 1 and by_row != values.stride(0) or k > 1 and (by_entry != 1 or values.stride(1) != 1):
             raise ValueError("ids, values: rows must be contiguous and stand equally far apart")
         return _lib.Teacher(p, v, by_row if n > 1 else k, None if lse is None else self._packed(lse, "lse", T.f32, (n,)), k, temperature)
 

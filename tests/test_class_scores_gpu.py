@@ -702,3 +702,29 @@ def test_refusals(engine):
                  lambda: engine.top_device(x[:, ::2].t()[:, ::2].t(), 3), lambda: engine.distill_grad_device(x.t(), ids, vals, grad=torch.empty_like(x).t().half())):
         with pytest.raises(ddt.DDTError):
             call()
+
+
+def test_streams_of_another_device_are_refused(engine):
+    class Other:
+        device_index, cuda_stream = engine.device + 1, 0
+
+    x = matrix(3, 10, "fp32")
+    ids, vals, lse = engine.top_device(x, 2)
+    for call in (lambda: engine.adjust_device(x, out=torch.empty_like(x), stream=Other),
+                 lambda: engine.top_device(x, 2, ids=ids, values=vals, lse=lse, stream=Other),
+                 lambda: engine.distill_device(x.t(), ids, vals, loss=lse, stream=Other),
+                 lambda: engine.distill_grad_device(x.t(), ids, vals, loss=lse, grad=torch.empty(3, 10, device="cuda"), stream=Other)):
+        with pytest.raises(ValueError, match="stream"):
+            call()
+
+
+def test_teachers_of_one_entry_lie_in_any_order(engine):
+    """one entry per row: the distance of a row's entries says nothing"""
+    x = matrix(6, 10, "fp32").t()
+    ids, vals, _ = teacher_of(6, 10, 1, 1.0, ragged=False)
+    ids, vals = torch.from_numpy(ids).cuda(), torch.from_numpy(vals).cuda()
+    want = engine.distill_device(x, ids, vals)
+    assert torch.equal(engine.distill_device(x, ids.t().contiguous().t(), vals), want)
+    wide = torch.stack([vals, vals], 1)[:, 0]         # rows two apart, the ids' one apart
+    with pytest.raises(ValueError, match="equally far"):
+        engine.distill_device(x, ids, wide)
