@@ -246,25 +246,30 @@ __device__ __forceinline__ float penalise(float x, uint32_t w, const RowPenalty&
 // zeroes `words` counters (rounded up to 4) and counts the history of rows [r0, r0 + rows) for classes [c0, c0 + C) into
 // counts[r * row_pitch + c * class_pitch].  Integer LDS adds: their order does not show.  Offsets and class numbers come from the device
 // unchecked: offsets are clamped to the history's length, numbers outside the tile (also outside the matrix) count nowhere.
+template <uint32_t kAhead>
 __device__ __forceinline__ void count_history(const AdjustArgs& a, uint64_t r0, uint32_t rows, uint32_t c0, uint32_t C, uint32_t row_pitch,
                                               uint32_t class_pitch, uint32_t words, uint32_t* counts) {
-  __syncthreads();  // the tile before has been read
-  for (uint32_t i = threadIdx.x; i < (words + 3u) / 4u; i += blockDim.x) reinterpret_cast<uint4*>(counts)[i] = make_uint4(0u, 0u, 0u, 0u);
-  __syncthreads();
   const uint32_t waves = blockDim.x >> 6;
   const bool per_wave = rows >= waves;  // a wave per row; fewer rows than waves: all threads on one row after the other
   const uint32_t step = (per_wave ? 64u : blockDim.x) * 4u, start = (per_wave ? threadIdx.x & 63u : threadIdx.x) * 4u;
-  for (uint32_t r = per_wave ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0u; r < rows; r += per_wave ? waves : 1u) {
+  uint32_t r = per_wave ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0u;
+  int64_t lo, split, hi;
+  auto offsets = [&] {
     const int64_t len = (int64_t)a.history_len;
-    int64_t lo = a.first[r0 + r], hi = a.first[r0 + r + 1];
+    lo = a.first[r0 + r], hi = a.first[r0 + r + 1], split = a.prompt ? (int64_t)a.prompt[r0 + r] : 0;
     lo = lo < 0 ? 0 : lo > len ? len : lo;
     hi = hi < lo ? lo : hi > len ? len : hi;
-    int64_t split = a.prompt ? (int64_t)a.prompt[r0 + r] : 0;
     split = split < 0 ? lo : split > hi - lo ? hi : lo + split;
+  };
+  offsets();  // (r < rows) under way while the counters are cleared
+  __syncthreads();  // the tile before has been read
+  for (uint32_t i = threadIdx.x; i < (words + 3u) / 4u; i += blockDim.x) reinterpret_cast<uint4*>(counts)[i] = make_uint4(0u, 0u, 0u, 0u);
+  __syncthreads();
+  while (r < rows) {
     uint32_t* row = counts + r * row_pitch;
     // kAhead 16-byte loads of a thread in flight: every tile of the row reads the whole history (from L2), and one entry at a time
-    // that is 400 dependent loads for 100,000 entries
-    constexpr uint32_t kAhead = 2;
+    // that is 400 dependent loads for 100,000 entries.  Four for the long histories of 1024 threads (50,000 entries a row 21.7 -> 20.8 us),
+    // two elsewhere (four: 4096 entries a row 19.1 -> 19.9 us, 64 entries 43 -> 49)
     auto count_part = [&](int64_t from, int64_t to, bool in_prompt) {
       for (; from < to; from += 1 << 30) {  // (32-bit positions inside a piece)
         const int32_t* h = a.history + from;
@@ -293,6 +298,8 @@ __device__ __forceinline__ void count_history(const AdjustArgs& a, uint64_t r0, 
     };
     count_part(lo, split, true);
     count_part(split, hi, false);
+    r += per_wave ? waves : 1u;
+    if (r < rows) offsets();
   }
   __syncthreads();
 }
@@ -345,7 +352,7 @@ __global__ __launch_bounds__(NT) void adjust_rows_kernel(const AdjustArgs a, con
         }
       }
     }
-    if (HIST) count_history(a, r0, rows, c0, C, t.classes, 1u, rows * t.classes, lds_words);
+    if (HIST) count_history<NT == 1024 ? 4 : 2>(a, r0, rows, c0, C, t.classes, 1u, rows * t.classes, lds_words);
 #pragma unroll
     for (int u = 0; u < ITER; ++u) {
       if (q[u] >= rows || cl[u] >= C) continue;
@@ -385,7 +392,7 @@ __global__ __launch_bounds__(256) void adjust_classes_kernel(const AdjustArgs a,
     const uint32_t c0 = (uint32_t)(tile - rt * t.class_tiles) * t.classes;
     const uint32_t rows = (uint32_t)(a.n - r0 < t.rows ? a.n - r0 : t.rows);
     const uint32_t C = a.K - c0 < t.classes ? a.K - c0 : t.classes;
-    if (HIST) count_history(a, r0, rows, c0, C, 1u, t.rows, C * t.rows, lds_words);
+    if (HIST) count_history<2>(a, r0, rows, c0, C, 1u, t.rows, C * t.rows, lds_words);
     for (uint32_t idx = threadIdx.x; idx < (C << rp_log2); idx += 256u) {
       const uint32_t cl = idx >> rp_log2, rl = (idx & (rp - 1u)) * N, c = c0 + cl;
       if (rl >= rows) continue;
