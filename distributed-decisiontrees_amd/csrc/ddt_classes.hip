@@ -464,8 +464,9 @@ struct ExpSum {
   }
 };
 // The same, one instruction per score less, for the long rows: exponentials of fma(x, c, -r) with r an fp32 number a step or two above
-// m c -- never below it, where 2^(m c - r) of a large score's rounding would overflow.  finish() puts the difference right.  Where that rounding is no longer small against 1 (a largest score beyond 10^6 T, or a row without any,
-// whose m is the lowest number) it asks for the sum in the plain form instead.
+// m c -- never below it, where 2^(m c - r) of a large score's rounding would overflow.  finish() puts the difference right.  Where that
+// rounding is no longer small against 1 (a largest score beyond 10^6 T, or a row without any, whose m is the lowest number) it asks for
+// the sum in the plain form instead.
 constexpr float kPlainBeyond = 0x1p20f;
 struct RunSum {
   float m = -FLT_MAX, r, s = 0.f;
@@ -533,8 +534,9 @@ __device__ __forceinline__ void write_nothing(const TopArgs& a, uint64_t row, ui
   a.values[row * a.k + rank] = -kInf;
 }
 
-// few classes, few of them wanted: a thread per row, the best k = KK in registers (4 M x 10 fp32 class-major, k = 3: 52 us for 272 MB, 5.2 TB/s).  Row-major rows are staged in LDS (coalesced loads;
-// the row pitch is an odd number of words), class-major ones are coalesced as they are.
+// few classes, few of them wanted: a thread per row, the best k = KK in registers (4 M x 10 fp32 class-major, k = 3: 49 us for 272 MB,
+// 5.6 TB/s).  Row-major rows are staged in LDS (coalesced loads; the row pitch is an odd number of words), class-major ones are coalesced
+// as they are.
 template <class T>
 __device__ __forceinline__ uint32_t staged_pitch(uint32_t K) {  // elements
   constexpr uint32_t per_word = 4 / sizeof(T);
@@ -1211,8 +1213,9 @@ __host__ __device__ constexpr uint32_t distill_words(uint32_t K, uint32_t k, uin
   return (Entries::words(k) + 4u + 2u * ((threads + 63u) / 64u) + (K + 31u) / 32u + 1u) & ~1u;
 }
 
-// NT threads per row: 16 (4 rows per wave: what a row does once costs a fourth of a wave), 64 (a wave) or the whole block.  P > 0: the row's packs stay in registers, P per thread,
-// all of them loaded at once while the teacher's entries are fetched, so that the gradient costs one read and one write of the matrix.
+// NT threads per row: 16 (4 rows per wave: what a row does once costs a fourth of a wave), 64 (a wave) or the whole block.  P > 0: the
+// row's packs stay in registers, P per thread, all of them loaded at once while the teacher's entries are fetched, so that the gradient
+// costs one read and one write of the matrix.
 // P = 0 (rows of more than 512 x 32 packs): the row is read a second time for the gradient, from whichever cache still holds it.
 // S is a bitmap in LDS, a pack's bits next to each other.
 template <class T, int NT, int P, bool GRAD>
@@ -1424,9 +1427,10 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void distill_kernel(const Dist
   }
 }
 
-// up to 32 classes: a thread per row, rows staged in LDS and their gradients collected there in fp32.  1 M x 10 fp32, k = 4: 47 us, 1150
-// vector instructions per wave of 64 rows (30 us' worth of issue): the 64-bit numbers of the rows bound it, not the 120 MB.  KK > 0: k = KK entries per row,
-// in registers with their exponentials; KK = 0: any number, read and computed again where they are needed.
+// up to 32 classes: a thread per row, rows staged in LDS and their gradients collected there in fp32.  1 M x 10 fp32, k = 4: 46 us, 1150
+// vector instructions per wave of 64 rows (30 us' worth of issue): the 64-bit numbers of the rows bound it, not the 120 MB.  KK > 0:
+// k = KK entries per row, in registers with their exponentials; KK = 0: any number, read and computed again where they are needed.
+// (Up to KK = 5, 124 registers and four waves per SIMD; without the branches on entries it is 135 and 52 -> 56 us.)
 template <class T, int KK, bool GRAD>
 __global__ __launch_bounds__(256) void distill_thread_kernel(const DistillArgs a) {
   T* stage = reinterpret_cast<T*>(lds_words);
