@@ -117,6 +117,7 @@ def _torch_types():
         raw = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
         _types = types.SimpleNamespace(
             torch=torch, f32=torch.float32, i32=torch.int32, u32=torch.uint32, i64=torch.int64, raw_stream=raw,
+            grad_enabled=torch.is_grad_enabled, wrote=torch.autograd.graph.increment_version,
             codes={torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
     return _types
 
@@ -255,6 +256,9 @@ class Engine:
     # logits.t() (a view: the strides say which it is).  Everything is asynchronous on `stream` (default: the device's current
     # one); results that are not handed in are allocated on it.  The checks are written for the calls that take less time on the
     # device than in Python: no context, device or dtype object is made on the way through.
+    # No gradient goes through adjust_device, top_device and distill*_device (distill is the call with one): a result that autograd
+    # would have to see written is refused, and every caller's tensor that is written counts as modified in place (_version), so that
+    # a backward pass that saved it says so.
     def _tensor(self, t, what: str, dtype, shape=None) -> int:
         if not t.is_cuda or t.get_device() != self.device:
             raise ValueError(f"{what}: on {t.device}, the engine is on cuda:{self.device}")
@@ -269,6 +273,13 @@ class Engine:
         if not t.is_contiguous():
             raise ValueError(f"{what}: must be contiguous")
         return p
+
+    @staticmethod
+    def _result(t, what: str):
+        """a caller's tensor that the call writes"""
+        if t.requires_grad and _torch_types().grad_enabled():
+            raise ValueError(f"{what}: requires grad and would be written without autograd's knowledge (torch.no_grad(), or detach it)")
+        return t
 
     def _scores(self, t, what: str, rows: int = 1) -> _lib.Scores:
         """ddt_scores_t of a tensor whose dimension `rows` counts the rows"""
@@ -351,14 +362,17 @@ class Engine:
                 a.presence = self._packed(presence, "presence", T.f32, (n,))
         elif not (history_first is None and history_prompt is None and repetition is None and frequency is None and presence is None):
             raise ValueError("history_first, history_prompt and penalties need a history")
+        given = out
         if out is None:
             row_major = s.class_stride == 1 and (s.row_stride >= K or n <= 1)
             new = self._allocator(class_scores, stream)
             out = new((n, K)).t() if row_major else new((K, n))
             o = _lib.Scores(out.data_ptr(), n, K if row_major else 1, 1 if row_major else n, K, s.dtype)
         else:
-            o = self._scores(out, "out")
+            o = self._scores(self._result(out, "out"), "out")
         self._check(self._L.ddt_adjust_scores_device(self._h, C.byref(s), C.byref(a), C.byref(o), self._stream(stream)))
+        if given is not None:
+            T.wrote(given)
         return out
 
     def top_device(self, class_scores, k: int, temperature: float = 1.0, ids=None, values=None, lse=None, stream=None):
@@ -369,23 +383,26 @@ class Engine:
         T = _torch_types()
         s = self._scores(class_scores, "class_scores")
         n = s.rows
+        given = [t for t in (ids, values, lse) if t is not None]
         new = self._allocator(class_scores, stream)
         if ids is None:
             ids = new((n, k), dtype=T.i32)
             p_ids = ids.data_ptr()
         else:
-            p_ids = self._packed(ids, "ids", T.i32, (n, k))
+            p_ids = self._packed(self._result(ids, "ids"), "ids", T.i32, (n, k))
         if values is None:
             values = new((n, k), dtype=T.f32)
             p_values = values.data_ptr()
         else:
-            p_values = self._packed(values, "values", T.f32, (n, k))
+            p_values = self._packed(self._result(values, "values"), "values", T.f32, (n, k))
         if lse is None:
             lse = new((n,), dtype=T.f32)
             p_lse = lse.data_ptr()
         else:
-            p_lse = self._packed(lse, "lse", T.f32, (n,))
+            p_lse = self._packed(self._result(lse, "lse"), "lse", T.f32, (n,))
         self._check(self._L.ddt_top_scores_device(self._h, C.byref(s), k, temperature, p_ids, p_values, p_lse, self._stream(stream)))
+        if given:
+            T.wrote(given)
         return ids, values, lse
 
     def top_classes_device(self, d_tuples, k: int, temperature: float = 1.0, stream=None, **adjust):
@@ -418,12 +435,15 @@ class Engine:
         T = _torch_types()
         s = self._scores(student, "student", rows=0)
         t = self._teacher(s.rows, ids, values, lse, temperature)
+        given = loss
         if loss is None:
             loss = self._allocator(student, stream)((s.rows,), dtype=T.f32)
             p_loss = loss.data_ptr()
         else:
-            p_loss = self._packed(loss, "loss", T.f32, (s.rows,))
+            p_loss = self._packed(self._result(loss, "loss"), "loss", T.f32, (s.rows,))
         self._check(self._L.ddt_distill_device(self._h, C.byref(s), C.byref(t), p_loss, self._stream(stream)))
+        if given is not None:
+            T.wrote(given)
         return loss
 
     def distill_grad_device(self, student, ids, values, lse=None, row_weight=None, temperature: float = 1.0, loss=None, grad=None,
@@ -438,18 +458,21 @@ class Engine:
         w, w_stride = None, 0
         if row_weight is not None:
             w, w_stride = self._tensor(row_weight, "row_weight", T.f32, (n,)), row_weight.stride(0) if n > 1 else 0
+        given = [t for t in (loss, grad) if t is not None]
         new = self._allocator(student, stream)
         if loss is None:
             loss = new((n,), dtype=T.f32)
             p_loss = loss.data_ptr()
         else:
-            p_loss = self._packed(loss, "loss", T.f32, (n,))
+            p_loss = self._packed(self._result(loss, "loss"), "loss", T.f32, (n,))
         if grad is None:
             grad = new((n, s.num_classes))
             g = _lib.Scores(grad.data_ptr(), n, s.num_classes, 1, s.num_classes, s.dtype)
         else:
-            g = self._scores(grad, "grad", rows=0)
+            g = self._scores(self._result(grad, "grad"), "grad", rows=0)
         self._check(self._L.ddt_distill_grad_device(self._h, C.byref(s), C.byref(t), w, w_stride, p_loss, C.byref(g), self._stream(stream)))
+        if given:
+            T.wrote(given)
         return loss, grad
 
     def distill(self, student, ids, values, lse=None, temperature: float = 1.0):
