@@ -9,6 +9,8 @@
 #include <float.h>
 #include <math.h>
 
+#include <type_traits>
+
 #include "../../include/ddt.h"
 #include "ddt_classes.h"
 
@@ -121,7 +123,7 @@ __device__ __forceinline__ uint32_t forgotten(uint32_t v) {
   return v;
 }
 
-// x ^ 2: the hardware instruction (1 ulp; results below 2^-126 may come back as 0 -- nothing next to a sum whose largest term is 1)
+// 2 ^ x: the hardware instruction (1 ulp; results below 2^-126 may come back as 0 -- nothing next to a sum whose largest term is 1)
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // 2^y and ln v beyond fp32 for the rows' own numbers.  2^y: y = n + f with |f| <= 1/2, the power series of e^(f ln 2) to the 10th power in
@@ -440,27 +442,39 @@ __global__ __launch_bounds__(256) void adjust_classes_kernel(const AdjustArgs a,
 // ---------------------------------------------------------------------------------------------------
 // sums of exponentials: (m, s) = (largest score so far, sum of exp((x - m) / T)).  The difference is taken before the scaling: it is
 // finite for finite scores (a row filled with the type's lowest value among them), and small, so exact enough, where it counts.
+// A thread's sum runs in 64 bits where its length grows with the row's: fp32 sums of near numbers are all rounded to the same side (one
+// score ahead of 2000 alike, added one by one: 500 half steps; 4000: 1000), and they are only as short as the groups that are added here.
 // ---------------------------------------------------------------------------------------------------
+// of up to 32 exponentials: four chains
+template <uint32_t N, class F>
+__device__ __forceinline__ float sum_of(F f) {
+  float t[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (uint32_t i = 0; i < N; ++i) t[i & 3u] += f(i);
+  return (t[0] + t[1]) + (t[2] + t[3]);
+}
 struct ExpSum {
   float m = -FLT_MAX, s = 0.f;
+  __device__ __forceinline__ void reduce_wave(float c) {  // the same in every lane afterwards
+    const float M = wave_max(m);
+    s = wave_sum(s * exp2_fast((m - M) * c));
+    m = M;
+  }
+};
+// a whole row in one thread, N scores at a time
+struct ThreadSum {
+  float m = -FLT_MAX;
+  double s = 0.0;
   template <uint32_t N>
   __device__ __forceinline__ void add(const float (&x)[N], float c) {
     float pm = x[0];
 #pragma unroll
     for (uint32_t i = 1; i < N; ++i) pm = fmaxf(pm, x[i]);
     if (pm > m) {
-      s *= exp2_fast((m - pm) * c);
+      s *= (double)exp2_fast((m - pm) * c);
       m = pm;
     }
-    float t = 0.f;
-#pragma unroll
-    for (uint32_t i = 0; i < N; ++i) t += exp2_fast((x[i] - m) * c);
-    s += t;
-  }
-  __device__ __forceinline__ void reduce_wave(float c) {  // the same in every lane afterwards
-    const float M = wave_max(m);
-    s = wave_sum(s * exp2_fast((m - M) * c));
-    m = M;
+    s += (double)sum_of<N>([&](uint32_t i) { return exp2_fast((x[i] - m) * c); });
   }
 };
 // The same, one instruction per score less, for the long rows: exponentials of fma(x, c, -r) with r an fp32 number a step or two above
@@ -468,8 +482,10 @@ struct ExpSum {
 // rounding is no longer small against 1 (a largest score beyond 10^6 T, or a row without any, whose m is the lowest number) it asks for
 // the sum in the plain form instead.
 constexpr float kPlainBeyond = 0x1p20f;
+template <class S>  // double; float for at most four groups
 struct RunSum {
-  float m = -FLT_MAX, r, s = 0.f;
+  float m = -FLT_MAX, r;
+  S s = 0;
   __device__ __forceinline__ explicit RunSum(float c) : r(reference(-FLT_MAX, c)) {}
   static __device__ __forceinline__ float reference(float m, float c) {
     return fminf(fmaxf(fmaf(fabsf(m * c), 0x1p-23f, m * c), -FLT_MAX), FLT_MAX);
@@ -481,13 +497,10 @@ struct RunSum {
     for (uint32_t i = 1; i < M; ++i) pm = fmaxf(pm, x[i]);
     if (pm > m) {
       const float nr = reference(pm, c);
-      s *= exp2_fast(r - nr);
+      s *= (S)exp2_fast(r - nr);
       m = pm, r = nr;
     }
-    float t[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (uint32_t i = 0; i < M; ++i) t[i & 3u] += exp2_fast(fmaf(x[i], c, -r));
-    s += (t[0] + t[1]) + (t[2] + t[3]);
+    s += (S)sum_of<M>([&](uint32_t i) { return exp2_fast(fmaf(x[i], c, -r)); });
     return pm;
   }
   // over the wave, or 16 lanes of it; plain(M) = this lane's sum of exp2((x - M) c)
@@ -497,14 +510,15 @@ struct RunSum {
     e.m = lanes_max<LANES>(m);
     if (fabsf(e.m * c) <= kPlainBeyond) {
       const float R = reference(e.m, c);
-      e.s = lanes_sum<LANES>(s * exp2_fast(r - R)) * exp2_fast((float)fma((double)e.m, -(double)c, (double)R));
+      e.s = lanes_sum<LANES>((float)s * exp2_fast(r - R)) * exp2_fast((float)fma((double)e.m, -(double)c, (double)R));
     } else {
       e.s = lanes_sum<LANES>(plain(e.m));
     }
     return e;
   }
 };
-__device__ __forceinline__ float log_sum(const ExpSum& e, double inv_T) {
+template <class Sum>
+__device__ __forceinline__ float log_sum(const Sum& e, double inv_T) {
   if (e.m == kInf) return kInf;
   return (float)((double)e.m * inv_T + log_64((double)e.s));  // nothing but -inf: log 0 = -inf
 }
@@ -589,19 +603,19 @@ __global__ __launch_bounds__(256) void top_thread_kernel(const TopArgs a) {
     int32_t id[KK];
 #pragma unroll
     for (int j = 0; j < KK; ++j) v[j] = -kInf, id[j] = -1;
-    ExpSum e;
-    constexpr uint32_t kAhead = CM ? 8 : 1;  // class-major: that many classes' loads of a row in flight
+    ThreadSum e;
+    constexpr uint32_t kAhead = 8;  // scores of a row that are summed together; class-major: their loads in flight
     for (uint32_t c0 = 0; c0 < a.K; c0 += kAhead) {
       T next[kAhead];
 #pragma unroll
-      for (uint32_t i = 0; i < kAhead; ++i)
-        if (c0 + i < a.K) next[i] = CM ? in[(c0 + i) * a.stride + row] : stage[tid * pitch + c0 + i];
+      for (uint32_t i = 0; i < kAhead; ++i) next[i] = c0 + i >= a.K ? (T)-kInf : CM ? in[(c0 + i) * a.stride + row] : stage[tid * pitch + c0 + i];
+      float xs[kAhead];
+#pragma unroll
+      for (uint32_t i = 0; i < kAhead; ++i) xs[i] = (float)next[i];
+      e.add(xs, c2);
 #pragma unroll
       for (uint32_t i = 0; i < kAhead; ++i) {
-        if (c0 + i >= a.K) break;
-        const float x1[1] = {(float)next[i]};
-        e.add(x1, c2);
-        float x = x1[0];
+        float x = xs[i];
         if (x > v[KK - 1]) {  // (false for NaN and -inf)
           int32_t xi = (int32_t)(c0 + i);
           bool placed = false;
@@ -948,7 +962,7 @@ __global__ __launch_bounds__(NT) void top_block_kernel(const TopArgs a) {
   for (uint64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
     const T* in = static_cast<const T*>(a.in) + row * a.stride;
     const uint32_t tid = forgotten(threadIdx.x), lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    RunSum run(c2);
+    RunSum<double> run(c2);
     float largest = -kInf;  // of the group
     uint32_t p0 = 0, groups = 0, left = per_group;
     __syncthreads();  // the row before is written
@@ -979,14 +993,13 @@ __global__ __launch_bounds__(NT) void top_block_kernel(const TopArgs a) {
     }
     const uint32_t best = score_key(run.m);  // (a thread without a candidate counts with the lowest score: the bound only sinks)
     const ExpSum e = run.finish<64>(c2, [&](float M) {
-      float t = 0.f;
+      double t = 0.0;
       for (uint32_t p = tid; p < packs; p += NT) {
         float x[N];
         load_pack(in, p * N, a.K, -kInf, x);
-#pragma unroll
-        for (uint32_t i = 0; i < N; ++i) t += exp2_fast((x[i] - M) * c2);
+        t += (double)sum_of<N>([&](uint32_t i) { return exp2_fast((x[i] - M) * c2); });
       }
-      return t;
+      return (float)t;
     });
     const bool quads = a.k <= NT / 8u;  // few wanted: the largest of four lanes will do, and is a quarter to search
     if (quads) {
@@ -1296,7 +1309,8 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void distill_kernel(const Dist
         sync();
       }
     }
-    RunSum run(c2);
+    typedef std::conditional_t<P == 0, double, float> Sum;
+    RunSum<Sum> run(c2);
     uint32_t holds = 0u;  // packs (of the registers) that hold a listed class
     if (P > 0) {
       constexpr int C = P < 4 ? P : 4;  // packs that are summed at a time
@@ -1342,15 +1356,14 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void distill_kernel(const Dist
       }
     }
     ExpSum o = run.template finish<NT < 64 ? NT : 64>(c2, [&](float M) {
-      float t = 0.f;
+      Sum t = 0;
       for (uint32_t p = tid; p < packs; p += NT) {
         float x[N];
         load_pack(in, p * N, a.K, -kInf, x);
         const uint32_t bits = listed_bits(p);
-#pragma unroll
-        for (uint32_t i = 0; i < N; ++i) t += (bits >> i) & 1u ? 0.f : exp2_fast((x[i] - M) * c2);
+        t += (Sum)sum_of<N>([&](uint32_t i) { return (bits >> i) & 1u ? 0.f : exp2_fast((x[i] - M) * c2); });
       }
-      return t;
+      return (float)t;
     });
     if (NT > 64 && tid < a.k) en.x[tid] = my_x;
     if (NT > 64) {
