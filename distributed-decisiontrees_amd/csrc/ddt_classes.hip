@@ -1149,6 +1149,10 @@ __global__ __launch_bounds__(NT) void top_block_kernel(const TopArgs a) {
 // The sums are kept apart because 1 - sum_S p and a loss near zero are differences of near numbers: p_R comes from its own sum, and an
 // error of s_o moves all p together so that it enters the loss times (p_R - q_R) only.
 // ---------------------------------------------------------------------------------------------------
+// Is the teacher's rest 1 - Q more than the rounding of its log-sum-exp (half a step, and 200 of them in the sum that it came from)?  Asked
+// only where the student has no probability for it: the loss is infinite then, and no loss at all if the teacher's rest is 0.
+__device__ __forceinline__ bool rest_counts(double Q, float lse) { return (float)(1.0 - Q) > (256.f + fabsf(lse)) * 0x1p-24f; }
+
 // what the gradient's pass over the row needs: grad = coef * exp((x - m) / T) outside S
 struct RowGrad {
   float m, coef;
@@ -1167,9 +1171,9 @@ struct Entries {
   static __host__ __device__ constexpr uint32_t words(uint32_t k) { return 7u * k; }
 };
 
-// one wave (or L = 16 lanes of it), one row: the teacher's entries against the student's row.  o = sums outside S.
+// one wave (or L = 16 lanes of it), one row: the teacher's entries against the student's row.  o = sums outside S, a bitmap.
 template <class T, int L, bool GRAD>
-__device__ __forceinline__ RowGrad row_loss(const DistillArgs& a, uint64_t row, const Entries& en, uint32_t lane, const ExpSum& o) {
+__device__ __forceinline__ RowGrad row_loss(const DistillArgs& a, uint64_t row, const Entries& en, const uint32_t* S, uint32_t lane, const ExpSum& o) {
   // the student's scale is the fp32 one of the sums outside S, for all its classes: p stays a softmax, of a temperature off by 2^-25
   const double inv_T = a.inv_T, x_scale = (double)a.scale;
   constexpr double kLn2 = 0.69314718055994530942;
@@ -1203,7 +1207,15 @@ __device__ __forceinline__ RowGrad row_loss(const DistillArgs& a, uint64_t row, 
   }
   // a student's row without a softmax (NaN, +inf, or nothing but -inf), or a teacher's: also where no entry's probability carries it on
   const bool none = !(Z > 0.0 && Q >= 0.0 && Q < __builtin_inf());
-  if (a.loss && lane == 0u) a.loss[row] = none ? __builtin_nanf("") : (float)loss;
+  if (a.loss && lane == 0u) {
+    float v = none ? __builtin_nanf("") : (float)loss;
+    if (o.s == 0.f && a.lse && rest_counts(Q, a.lse[row])) {
+      uint32_t listed = 0u;
+      for (uint32_t i = 0; a.K <= a.k && i < (a.K + 31u) / 32u; ++i) listed += __popc(S[i]);
+      if (listed < a.K) v += kInf;
+    }
+    a.loss[row] = v;
+  }
   RowGrad g = {o.m, 0.f};
   if (GRAD) {
     const double w = (a.weight ? (double)a.weight[row * a.weight_stride] : 1.0) * inv_T;
@@ -1375,7 +1387,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void distill_kernel(const Dist
         o.m = lane < kWaves ? part[2 * lane] : -FLT_MAX, o.s = lane < kWaves ? part[2 * lane + 1] : 0.f;
         o.reduce_wave(c2);
       }
-      const RowGrad g = row_loss<T, (NT < 64 ? NT : 64), GRAD>(a, row, en, lane, o);
+      const RowGrad g = row_loss<T, (NT < 64 ? NT : 64), GRAD>(a, row, en, bitmap, lane, o);
       if (GRAD && lane == 0u) ctl[2] = __float_as_uint(g.m), ctl[3] = __float_as_uint(g.coef);
     }
     if (GRAD) {
@@ -1444,8 +1456,9 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void distill_kernel(const Dist
 // vector instructions per wave of 64 rows (30 us' worth of issue): the 64-bit numbers of the rows bound it, not the 120 MB.  KK > 0:
 // k = KK entries per row, in registers with their exponentials; KK = 0: any number, read and computed again where they are needed.
 // (Up to KK = 5, 124 registers and four waves per SIMD; without the branches on entries it is 135 and 52 -> 56 us.)
+// (KK = 2 is held to the 96 registers of five waves: a register more cost 1 M x 10 bf16 39 -> 42 us.)
 template <class T, int KK, bool GRAD>
-__global__ __launch_bounds__(256) void distill_thread_kernel(const DistillArgs a) {
+__global__ __launch_bounds__(256, KK == 2 ? 5 : 1) void distill_thread_kernel(const DistillArgs a) {
   T* stage = reinterpret_cast<T*>(lds_words);
   const uint32_t pitch = staged_pitch<T>(a.K), gpitch = a.K | 1u;
   float* gstage = reinterpret_cast<float*>(lds_words + (256u * pitch * sizeof(T)) / 4u);
@@ -1525,6 +1538,8 @@ __global__ __launch_bounds__(256) void distill_thread_kernel(const DistillArgs a
           rest_s = (1.0 - Q) * inverse_64((double)os);
           loss = (1.0 - Q) * (log_64(rest_s) - (((double)om - (double)M) * x_scale * kLn2 - log_Z));
           Q = 1.0;
+        } else if (a.lse && os == 0.f && (uint32_t)__popc(listed) < a.K && rest_counts(Q, (float)shift)) {
+          loss = __builtin_inf();
         }
         const bool none = !(Z > 0.0 && Q >= 0.0 && Q < __builtin_inf());  // (as in row_loss)
         const double w = (double)weight * inv_T, p_scale = none ? __builtin_nan("") : Q * inverse_64(Z);

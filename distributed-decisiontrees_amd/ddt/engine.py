@@ -431,7 +431,8 @@ class Engine:
     def distill_device(self, student, ids, values, lse=None, temperature: float = 1.0, loss=None, stream=None):
         """KL divergence of a student's softmax (scores [n, K], row-major) from a teacher's top scores (ids, values, lse of
         top_device at the same temperature) -> loss fp32 [n].  lse None: the teacher's probabilities are normalised over the
-        listed classes; otherwise everything it does not list is one more outcome.  (ddt_distill_device)"""
+        listed classes; otherwise everything it does not list is one more outcome.  +inf where the teacher has a probability and the
+        student, at -inf, has none.  (ddt_distill_device)"""
         T = _torch_types()
         s = self._scores(student, "student", rows=0)
         t = self._teacher(s.rows, ids, values, lse, temperature)

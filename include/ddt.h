@@ -250,7 +250,10 @@ typedef struct ddt_teacher_t {
 } ddt_teacher_t;
 /* Distillation loss of a student's scores (row-major), p = softmax(student / T):
  *      loss[r] = sum_j q_j (log q_j - log p_(id j)) + q_R (log q_R - log p_R),   p_R = the student's probability of the classes not listed
- * The rest is left out where q_R or p_R is 0.  A row without entries: 0.  A class listed twice counts with both entries.  A row of the
+ * The rest is left out where q_R is 0 or every class is listed.  A probability q > 0 for which the student has none -- a listed class, or
+ * all classes not listed, at -inf -- makes the loss +inf; a q_R within the rounding of lse, (256 + |lse|) 2^-24, counts as 0 there.  The
+ * gradient then is that of p = 0 for a listed class, and of the loss without the rest (Q = sum q_j) where p_R is 0.  A row without
+ * entries: 0.  A class listed twice counts with both entries.  A row of the
  * student that holds NaN or +inf, or nothing but -inf, has no softmax: its loss and gradient are NaN.  So are those of a row whose teacher
  * has none (NaN or +inf among its entries; without lse nothing but -inf).
  * ..._grad: also grad (row-major, the student's type; may be the student's own buffer) =
