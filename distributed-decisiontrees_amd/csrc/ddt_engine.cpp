@@ -7,6 +7,8 @@
 // rtl/DTEngine/PCIeReceiver.sv:136-139,230-312; line packing rtl/DTEngine/core/PipelinedMUX.sv:65;
 // model store rtl/DTEngine/core/DTPU.sv:282-354; result packing rtl/DTEngine/ResultsCombiner.sv:136-160.
 #include <hip/hip_runtime.h>
+#include <sys/mman.h>
+#include <unistd.h>
 
 #include <algorithm>
 #include <chrono>
@@ -843,7 +845,7 @@ static void parallel_copy(ddt_engine* e, void* dst, const void* src, size_t byte
 static bool host_registered(const ddt_engine* e, const void* p, size_t bytes) {
   const char* q = static_cast<const char*>(p);
   for (const auto& r : e->pinned)
-    if (q >= static_cast<const char*>(r.first) && q + bytes <= static_cast<const char*>(r.first) + r.second) return true;
+    if (q >= static_cast<const char*>(r.first) && bytes <= r.second && (size_t)(q - static_cast<const char*>(r.first)) <= r.second - bytes) return true;
   return false;
 }
 
@@ -915,9 +917,16 @@ static int score_host(ddt_engine* e, const void* tuple_lines, size_t n, float* s
   return DDT_OK;
 }
 
+// is all of [p, p + bytes) memory of this process?  (msync with MS_ASYNC writes nothing; it answers ENOMEM for a page that is not there)
+static bool host_mapped(const void* p, size_t bytes) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p), page = a & ~((uintptr_t)sysconf(_SC_PAGESIZE) - 1);
+  return a + bytes > a && msync(reinterpret_cast<void*>(page), a + bytes - page, MS_ASYNC) == 0;
+}
+
 int ddt_host_register(ddt_engine* e, void* ptr, size_t bytes) {
   if (!e) return DDT_EINVAL;
   if (!ptr || !bytes) return fail(e, DDT_EINVAL, "ddt_host_register: NULL / empty range");
+  if (!host_mapped(ptr, bytes)) return fail(e, DDT_EINVAL, "ddt_host_register: %p, %zu bytes: not memory of this process", ptr, bytes);
   DeviceGuard dg(e->device);
   if (!dg.ok) return fail(e, DDT_EHIP, "hipSetDevice(%d) failed", e->device);
   for (const auto& r : e->pinned)
@@ -925,19 +934,23 @@ int ddt_host_register(ddt_engine* e, void* ptr, size_t bytes) {
   for (const void* p : e->refused)
     if (p == ptr) return fail(e, DDT_EINVAL, "ddt_host_register: %p is registered already", ptr);
   const hipError_t r = hipHostRegister(ptr, bytes, hipHostRegisterDefault);
+  if (r != hipSuccess) (void)hipGetLastError();
+  // "invalid value" for a range that is there (or "not supported"): a driver that does not pin memory that exists already
+  const bool staged = r == hipErrorInvalidValue || r == hipErrorNotSupported;
+  if (r != hipSuccess && !staged) return fail(e, DDT_EHIP, "hipHostRegister(%p, %zu) -> %s", ptr, bytes, hipGetErrorString(r));
   try {
-    if (r == hipSuccess) {
-      e->pinned.emplace_back(ptr, bytes);
-    } else {  // a machine whose driver does not pin memory that exists already: the range keeps going through the feeder's own pinned buffers
-      (void)hipGetLastError();
-      e->refused.push_back(ptr);
-      (void)fail(e, DDT_OK, "hipHostRegister(%p, %zu) -> %s: the range is staged as before", ptr, bytes, hipGetErrorString(r));
-    }
+    if (staged) e->refused.push_back(ptr);
+    else e->pinned.emplace_back(ptr, bytes);
   } catch (const std::bad_alloc&) {
-    if (r == hipSuccess) (void)hipHostUnregister(ptr);
+    if (!staged) (void)hipHostUnregister(ptr);
     return fail(e, DDT_ENOMEM, "ddt_host_register");
   }
   return DDT_OK;
+}
+
+int ddt_host_pinned(ddt_engine* e, const void* ptr, size_t bytes) {
+  if (!e) return DDT_EINVAL;
+  return host_registered(e, ptr, bytes) ? 1 : 0;
 }
 
 int ddt_host_unregister(ddt_engine* e, void* ptr) {

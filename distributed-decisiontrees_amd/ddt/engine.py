@@ -497,10 +497,16 @@ class Engine:
         self._check(self._L.ddt_score(self._h, t.ctypes.data, t.shape[0], out.ctypes.data))
         return out
 
-    def host_register(self, a: np.ndarray):
-        """Pin a host array for this engine's device (ddt_host_register): ddt_score then DMAs it directly."""
+    def host_register(self, a: np.ndarray) -> bool:
+        """Pin a host array for this engine's device (ddt_host_register): ddt_score then DMAs it directly.  -> is it pinned?  (A driver
+        that does not pin memory that exists already leaves it to be staged like any other.)"""
         assert a.flags.c_contiguous
         self._check(self._L.ddt_host_register(self._h, a.ctypes.data, a.nbytes))
+        return self.host_pinned(a)
+
+    def host_pinned(self, a: np.ndarray) -> bool:
+        """Does ddt_score move this array directly (ddt_host_pinned)?"""
+        return self._L.ddt_host_pinned(self._h, a.ctypes.data, a.nbytes) == 1
 
     def host_unregister(self, a: np.ndarray):
         self._check(self._L.ddt_host_unregister(self._h, a.ctypes.data))

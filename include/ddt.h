@@ -27,7 +27,7 @@
 extern "C" {
 #endif
 
-#define DDT_ABI_VERSION 7 /* 7: class-score operators (ddt_adjust_scores_device, ddt_top_scores_device, ddt_distill*_device); 6: ddt_info::build_checks (was reserved), "sparse_r_*" kernels + option sparse_r32, ddt_debug_rank32_tables; 5: ddt_info grew (fallback_kernel); 4: hybrid jobs (ddt_comm_create_hybrid, ddt_score_hybrid_device, ...), ddt_comm_abort; 3: ddt_stats grew */
+#define DDT_ABI_VERSION 8 /* 8: ddt_host_pinned; 7: class-score operators (ddt_adjust_scores_device, ddt_top_scores_device, ddt_distill*_device); 6: ddt_info::build_checks (was reserved), "sparse_r_*" kernels + option sparse_r32, ddt_debug_rank32_tables; 5: ddt_info grew (fallback_kernel); 4: hybrid jobs (ddt_comm_create_hybrid, ddt_score_hybrid_device, ...), ddt_comm_abort; 3: ddt_stats grew */
 
 /* Threading: an engine is not thread-safe -- calls on ONE engine must not overlap; different engines (also on the
  * same device) are independent.  ddt_*_device calls are asynchronous on the given stream; ddt_destroy and
@@ -145,9 +145,12 @@ int ddt_shard_range(uint32_t num_trees, uint32_t shard_index, uint32_t shard_cou
  *    ddt_host_register pins [ptr, ptr + bytes) for this engine's device (hipHostRegister); ddt_score / ddt_classify calls whose
  *    tuple buffer (and, for ddt_score, score buffer) lies inside a registered range then move the data with the DMA engine
  *    directly -- no staging copy through the engine's own pinned buffers.  Where the driver does not pin memory that exists already, the
- *    range is accepted and staged like any other (ddt_last_error then says so).  Unregister before freeing the memory.     -- */
+ *    range is accepted and staged like any other; ddt_host_pinned tells: 1 = [ptr, ptr + bytes) moves directly, 0 = it is staged.  A range
+ *    that is not all memory of this process is DDT_EINVAL, any other failure of the driver's DDT_EHIP.  Unregister before freeing the
+ *    memory.                                                                                                               -- */
 int ddt_host_register(ddt_engine* e, void* ptr, size_t bytes);
 int ddt_host_unregister(ddt_engine* e, void* ptr);
+int ddt_host_pinned(ddt_engine* e, const void* ptr, size_t bytes);
 
 /* Host buffers: tuple_lines = n_tuples * ceil(F/4) lines of 16 B; scores_out = n_tuples fp32.
  * Streams the batch through the pinned hipMemcpyAsync feeder (the PCIe feeder): three slots -- staging of chunk k+2 by host

@@ -13,7 +13,7 @@
 #define __forceinline__ inline
 
 typedef int hipError_t;
-enum { hipSuccess = 0, hipErrorInvalidValue = 1, hipErrorOutOfMemory = 2, hipErrorInvalidDevice = 101 };
+enum { hipSuccess = 0, hipErrorInvalidValue = 1, hipErrorOutOfMemory = 2, hipErrorInvalidDevice = 101, hipErrorHostMemoryAlreadyRegistered = 712, hipErrorNotSupported = 801 };
 struct MockStream;
 struct MockEvent;
 typedef MockStream* hipStream_t;

@@ -454,7 +454,8 @@ hipError_t hipHostFree(void* p) {
   free(p);
   return hipSuccess;
 }
-hipError_t hipHostRegister(void*, size_t, unsigned) { return hipSuccess; }
+static hipError_t g_pin_result = hipSuccess;  // what hipHostRegister answers (mock_pin_result)
+hipError_t hipHostRegister(void*, size_t, unsigned) { return g_pin_result; }
 hipError_t hipHostUnregister(void*) { return hipSuccess; }
 hipError_t hipEventCreate(hipEvent_t* e) { return hipEventCreateWithFlags(e, 0); }
 hipError_t hipEventSynchronize(hipEvent_t e) {
@@ -644,6 +645,7 @@ void mock_reset(int policy, uint64_t seed, int devices) {
   g_h2d_bytes = 0;
 }
 uint64_t mock_h2d_bytes(void) { return g_h2d_bytes; }
+void mock_pin_result(int r) { g_pin_result = r; }
 void mock_costs(double per_row, double per_float_moved, double per_float_copied) {
   std::lock_guard<std::mutex> lk(M);
   g_cost_row = per_row, g_cost_float = per_float_moved, g_cost_copy = per_float_copied;
