@@ -254,8 +254,10 @@ class Engine:
     # ---- class scores: after the trees ---------------------------------------------------------------
     # Matrices are torch tensors [num_classes, n] as classify_device returns them; row-major logits [n, num_classes] go in as
     # logits.t() (a view: the strides say which it is).  Everything is asynchronous on `stream` (default: the device's current
-    # one); results that are not handed in are allocated on it.  The checks are written for the calls that take less time on the
-    # device than in Python: no context, device or dtype object is made on the way through.
+    # one); results that are not handed in are allocated on it, so another stream that reads them waits for it first.  The caller's
+    # tensors may be let go right after a call: their memory is not given out again before `stream` is done with them.  The checks
+    # are written for the calls that take less time on the device than in Python: no context, device or dtype object is made on the
+    # way through.
     # No gradient goes through adjust_device, top_device and distill*_device (distill is the call with one): a result that autograd
     # would have to see written is refused, and every caller's tensor that is written counts as modified in place (_version), so that
     # a backward pass that saved it says so.
@@ -294,12 +296,15 @@ class Engine:
         c, d = t.stride()
         return _lib.Scores(t.data_ptr(), b, d, c, a, code) if rows else _lib.Scores(t.data_ptr(), a, c, d, b, code)
 
-    def _stream(self, stream):
-        """handle of the stream of a call"""
+    def _stream(self, stream, *used):
+        """handle of the stream of a call, which uses these tensors"""
         if stream is None:
             return _torch_types().raw_stream(self.device)
         if stream.device_index != self.device:
             raise ValueError(f"stream: of cuda:{stream.device_index}, the engine is on cuda:{self.device}")
+        for t in used:
+            if t is not None:
+                t.record_stream(stream)
         return stream.cuda_stream
 
     @staticmethod
@@ -370,7 +375,9 @@ class Engine:
             o = _lib.Scores(out.data_ptr(), n, K if row_major else 1, 1 if row_major else n, K, s.dtype)
         else:
             o = self._scores(self._result(out, "out"), "out")
-        self._check(self._L.ddt_adjust_scores_device(self._h, C.byref(s), C.byref(a), C.byref(o), self._stream(stream)))
+        self._check(self._L.ddt_adjust_scores_device(self._h, C.byref(s), C.byref(a), C.byref(o),
+                                                     self._stream(stream, class_scores, bias, allowed, history, history_first, history_prompt, repetition,
+                                                                  frequency, presence, out)))
         if given is not None:
             T.wrote(given)
         return out
@@ -400,7 +407,8 @@ class Engine:
             p_lse = lse.data_ptr()
         else:
             p_lse = self._packed(self._result(lse, "lse"), "lse", T.f32, (n,))
-        self._check(self._L.ddt_top_scores_device(self._h, C.byref(s), k, temperature, p_ids, p_values, p_lse, self._stream(stream)))
+        self._check(self._L.ddt_top_scores_device(self._h, C.byref(s), k, temperature, p_ids, p_values, p_lse,
+                                                  self._stream(stream, class_scores, ids, values, lse)))
         if given:
             T.wrote(given)
         return ids, values, lse
@@ -413,6 +421,7 @@ class Engine:
 
         import torch
 
+        self._stream(stream, d_tuples, *adjust.values())
         with contextlib.nullcontext() if stream is None else torch.cuda.stream(stream):
             _, scores = self.classify_device(d_tuples, want_labels=False)
             if adjust:
@@ -442,7 +451,8 @@ class Engine:
             p_loss = loss.data_ptr()
         else:
             p_loss = self._packed(self._result(loss, "loss"), "loss", T.f32, (s.rows,))
-        self._check(self._L.ddt_distill_device(self._h, C.byref(s), C.byref(t), p_loss, self._stream(stream)))
+        self._check(self._L.ddt_distill_device(self._h, C.byref(s), C.byref(t), p_loss,
+                                               self._stream(stream, student, ids, values, lse, loss)))
         if given is not None:
             T.wrote(given)
         return loss
@@ -471,7 +481,8 @@ class Engine:
             g = _lib.Scores(grad.data_ptr(), n, s.num_classes, 1, s.num_classes, s.dtype)
         else:
             g = self._scores(self._result(grad, "grad"), "grad", rows=0)
-        self._check(self._L.ddt_distill_grad_device(self._h, C.byref(s), C.byref(t), w, w_stride, p_loss, C.byref(g), self._stream(stream)))
+        self._check(self._L.ddt_distill_grad_device(self._h, C.byref(s), C.byref(t), w, w_stride, p_loss, C.byref(g),
+                                                    self._stream(stream, student, ids, values, lse, row_weight, loss, grad)))
         if given:
             T.wrote(given)
         return loss, grad
