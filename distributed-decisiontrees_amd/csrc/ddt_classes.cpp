@@ -18,14 +18,19 @@ struct Layout {
   uint64_t stride = 0;
 };
 
+bool fits(const ddt_scores_t* s, bool class_major) {
+  const uint64_t K = s->num_classes, n = s->rows;
+  if (class_major) return (s->row_stride == 1 || n <= 1) && (s->class_stride >= n || K == 1);
+  return (s->class_stride == 1 || K == 1) && (s->row_stride >= K || n <= 1);
+}
+
 int check_scores(ddt_engine* e, const char* what, const ddt_scores_t* s, int want_class_major, Layout* out) {
   if (!s) return fail(e, DDT_EINVAL, "%s: NULL matrix", what);
   if (s->dtype > DDT_BF16) return fail(e, DDT_EINVAL, "%s: dtype %u", what, s->dtype);
   if (s->num_classes == 0 || s->num_classes > DDT_MAX_CLASSES) return fail(e, DDT_EINVAL, "%s: %u classes", what, s->num_classes);
   const uint64_t K = s->num_classes, n = s->rows, limit = uint64_t(1) << 48;
   if (n > limit || s->row_stride > limit || s->class_stride > limit) return fail(e, DDT_EINVAL, "%s: shape out of range", what);
-  const bool row_major = (s->class_stride == 1 || K == 1) && (s->row_stride >= K || n <= 1);
-  const bool class_major = (s->row_stride == 1 || n <= 1) && (s->class_stride >= n || K == 1);
+  const bool row_major = fits(s, false), class_major = fits(s, true);
   if (!row_major && !class_major)
     return fail(e, DDT_EINVAL, "%s: strides %llu (rows), %llu (classes) are neither row-major nor class-major without overlap", what,
                 (unsigned long long)s->row_stride, (unsigned long long)s->class_stride);
@@ -107,16 +112,12 @@ int ddt_adjust_scores_device(ddt_engine* e, const ddt_scores_t* in, const ddt_ad
   int rc = check_scores(e, "scores", in, -1, &li);
   if (rc) return rc;
   if (!adj) return fail(e, DDT_EINVAL, "NULL adjustment");
-  rc = check_result(e, "adjusted scores", in, li, out, &lo);
-  if (rc && in->num_classes > 1 && in->rows > 1) return rc;
-  if (rc) {  // a single row or class is either layout: take the one that the result has
-    rc = check_scores(e, "adjusted scores", out, -1, &lo);
-    if (rc) return rc;
-    rc = check_scores(e, "scores", in, lo.class_major, &li);
-    if (rc) return rc;
-    rc = check_result(e, "adjusted scores", in, li, out, &lo);
+  if (out && !fits(out, li.class_major) && fits(out, !li.class_major) && fits(in, !li.class_major)) {  // a single row: take the result's layout
+    rc = check_scores(e, "scores", in, !li.class_major, &li);
     if (rc) return rc;
   }
+  rc = check_result(e, "adjusted scores", in, li, out, &lo);
+  if (rc) return rc;
   const uint64_t limit = uint64_t(1) << 48, words = (in->num_classes + 31u) / 32u;
   if (adj->bias && (adj->bias_row_stride > limit || adj->bias_class_stride > limit)) return fail(e, DDT_EINVAL, "bias: stride out of range");
   if (adj->allowed && adj->allowed_row_stride != 0 && (adj->allowed_row_stride < words || adj->allowed_row_stride > limit))
