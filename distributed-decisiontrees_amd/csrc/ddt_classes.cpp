@@ -78,7 +78,9 @@ int distill(ddt_engine* e, const ddt_scores_t* s, const ddt_teacher_t* t, const 
   if (rc) return rc;
   if (!t) return fail(e, DDT_EINVAL, "NULL teacher");
   if (t->k == 0 || t->k > DDT_MAX_TOP) return fail(e, DDT_EINVAL, "teacher: k %u (1 .. %u)", t->k, (unsigned)DDT_MAX_TOP);
-  if (t->row_stride < t->k && s->rows > 1) return fail(e, DDT_EINVAL, "teacher: row_stride below k");
+  if (s->rows > 1 && (t->row_stride < t->k || t->row_stride > (uint64_t(1) << 48)))
+    return fail(e, DDT_EINVAL, "teacher: row_stride %llu for k %u", (unsigned long long)t->row_stride, t->k);
+  if (weight && weight_stride > (uint64_t(1) << 48)) return fail(e, DDT_EINVAL, "row_weight: stride out of range");
   rc = check_temperature(e, t->temperature);
   if (rc) return rc;
   if (want_grad) {

@@ -198,7 +198,8 @@ int ddt_argmax_device(ddt_engine* e, const float* d_class_scores, uint32_t num_c
  *    1: class-major is what ddt_classify_device writes ([num_classes][n]: row_stride 1, class_stride n), row-major ([n][num_classes]:
  *    class_stride 1) is how a network holds its logits.  Strides may leave gaps, rows / classes must not overlap, data must be aligned to
  *    its element.  The calls need an engine (its device, its error text) but no loaded model, keep nothing, allocate nothing and only enqueue
- *    on `hip_stream`: they may be captured.  Whatever the type, sums and exponentials are fp32 or wider and a result is rounded once.     -- */
+ *    on `hip_stream`: they may be captured.  They leave the engine as it is, so unlike its other calls they may overlap on one engine (the
+ *    error text aside).  A result must not lie across anything else that its call reads or writes, but where a call says so.  Whatever the type, sums and exponentials are fp32 or wider and a result is rounded once.     -- */
 enum { DDT_FP32 = 0, DDT_FP16 = 1, DDT_BF16 = 2 };
 #define DDT_MAX_CLASSES (1u << 20)  /* classes these calls take */
 #define DDT_MAX_TOP 256             /* classes a teacher lists per row, and ddt_top_scores_device returns */
