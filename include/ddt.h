@@ -30,7 +30,8 @@ extern "C" {
 #define DDT_ABI_VERSION 8 /* 8: ddt_host_pinned; 7: class-score operators (ddt_adjust_scores_device, ddt_top_scores_device, ddt_distill*_device); 6: ddt_info::build_checks (was reserved), "sparse_r_*" kernels + option sparse_r32, ddt_debug_rank32_tables; 5: ddt_info grew (fallback_kernel); 4: hybrid jobs (ddt_comm_create_hybrid, ddt_score_hybrid_device, ...), ddt_comm_abort; 3: ddt_stats grew */
 
 /* Threading: an engine is not thread-safe -- calls on ONE engine must not overlap; different engines (also on the
- * same device) are independent.  ddt_*_device calls are asynchronous on the given stream; ddt_destroy and
+ * same device) are independent.  (The class-score calls leave the engine as it is: they may overlap with each other and with any
+ * call but ddt_destroy; only the error text is then whoever's failed last.)  ddt_*_device calls are asynchronous on the given stream; ddt_destroy and
  * ddt_load_model* wait for the device before freeing or replacing what such work may still read. */
 
 /* Return codes.  The reference has no error signalling beyond status counters (EngineCSR.sv:113-126);
@@ -198,8 +199,8 @@ int ddt_argmax_device(ddt_engine* e, const float* d_class_scores, uint32_t num_c
  *    1: class-major is what ddt_classify_device writes ([num_classes][n]: row_stride 1, class_stride n), row-major ([n][num_classes]:
  *    class_stride 1) is how a network holds its logits.  Strides may leave gaps, rows / classes must not overlap, data must be aligned to
  *    its element.  The calls need an engine (its device, its error text) but no loaded model, keep nothing, allocate nothing and only enqueue
- *    on `hip_stream`: they may be captured.  They leave the engine as it is, so unlike its other calls they may overlap on one engine (the
- *    error text aside).  A result must not lie across anything else that its call reads or writes, but where a call says so.  Whatever the type, sums and exponentials are fp32 or wider and a result is rounded once.     -- */
+ *    on `hip_stream`: they may be captured.  A result must not lie across anything else that its call reads or writes, but where a call says
+ *    so.  Whatever the type, sums and exponentials are fp32 or wider and a result is rounded once.                                        -- */
 enum { DDT_FP32 = 0, DDT_FP16 = 1, DDT_BF16 = 2 };
 #define DDT_MAX_CLASSES (1u << 20)  /* classes these calls take */
 #define DDT_MAX_TOP 256             /* classes a teacher lists per row, and ddt_top_scores_device returns */
