@@ -314,8 +314,9 @@ struct AdjustTiles {
 
 // Row-major: a tile is `rows` rows times `classes` classes, at most NT * ITER packs of them, ITER per thread.  All loads of a thread --
 // scores, bias, mask, the row's penalties -- are on their way before the history is counted.  What bounds it with a history is the chain of
-// a tile's latencies (offsets, entries, counters, scores): 64 x 128000 bf16 takes 11 us without histories, 14 with 10 entries a row, 18 with
-// 4096; 32 x 50257 fp32 with 50,000 entries a row 20 us, six rounds of loads for the longest row.
+// a tile's latencies (offsets, entries, counters, scores): 64 x 128000 bf16 takes 10 us without histories, 14 with 10 entries a row, 18 with
+// 4096; 32 x 50257 fp32 with 50,000 entries a row 20 us, six rounds of loads for the longest row.  A row's tiles lie on all eight XCDs, and
+// each of their L2s fetches the history for itself: 61 MB where scores and histories once are 13, 26 where they are 18.5.
 template <class T, bool HIST, int NT, int ITER>
 __global__ __launch_bounds__(NT) void adjust_rows_kernel(const AdjustArgs a, const AdjustTiles t) {
   constexpr uint32_t N = Pack<T>::N;
@@ -548,9 +549,9 @@ __device__ __forceinline__ void write_nothing(const TopArgs& a, uint64_t row, ui
   a.values[row * a.k + rank] = -kInf;
 }
 
-// few classes, few of them wanted: a thread per row, the best k = KK in registers (4 M x 10 fp32 class-major, k = 3: 49 us for 272 MB,
-// 5.6 TB/s).  Row-major rows are staged in LDS (coalesced loads; the row pitch is an odd number of words), class-major ones are coalesced
-// as they are.
+// few classes, few of them wanted: a thread per row, the best k = KK in registers (4 M x 10 fp32 class-major, k = 3: 49 us for 272 MB, 5.5
+// TB/s and 42 us' worth of vector issue).  Row-major rows are staged in LDS (coalesced loads; the row pitch is an odd number of words),
+// class-major ones are coalesced as they are.
 template <class T>
 __device__ __forceinline__ uint32_t staged_pitch(uint32_t K) {  // elements
   constexpr uint32_t per_word = 4 / sizeof(T);
@@ -806,9 +807,9 @@ __global__ __launch_bounds__(256) void top_lanes_kernel(const TopArgs a) {
   }
 }
 
-// up to 2048 classes: a wave per row, all its scores in registers (P packs per lane).  16384 x 1000 fp32, k = 20: 24 us; the 534 vector
-// instructions per row bound it (14 us' worth of issue), not the 65 MB.  Class-major rows are staged through LDS, 16 at a
-// time for the 8 waves of the block.
+// up to 2048 classes: a wave per row, all its scores in registers (P packs per lane).  16384 x 1000 fp32, k = 20: 24 us.  What bounds it is
+// neither the 65 MB nor the 519 vector instructions per row (14 us' worth of issue) but a wave's chain of dependent steps: the bits of the
+// bound, the list, the ranks.  Class-major rows are staged through LDS, 16 at a time for the 8 waves of the block.
 constexpr uint32_t kWaveList = 128;  // candidates that are ranked without an exact count
 __device__ __forceinline__ uint32_t lanes_below(uint64_t ballot) {
   return __builtin_amdgcn_mbcnt_hi((uint32_t)(ballot >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)ballot, 0u));
@@ -938,7 +939,8 @@ __global__ __launch_bounds__(top_wave_waves(CM) * 64) void top_wave_kernel(const
 // threads' maxima is a bound that at least k scores reach, and only the groups that reach it -- about k of them, 64 packs of
 // 128000 -- are read a second time to list the candidates.  Rows with more candidates than the list holds (scores that tie, or stand
 // in few threads) are narrowed down by counting, bit by bit, over the threads that reach the bound.
-// 512 x 128000 bf16, k = 64: 27 us for 131 MB; with a second look at every pack of the threads that hold candidates -- a cache line each, the
+// 512 x 128000 bf16, k = 64: 30 us for 131 MB, 22 of them reading at the 6 TB/s of a plain read; bound, second look and ranks of the two rows
+// of a CU come behind it with nothing to hide them.  With a second look at every pack of the threads that hold candidates -- a cache line each, the
 // whole row over -- it was 41.
 constexpr uint32_t kListCap = 1024, kGroups = 16;
 constexpr uint32_t top_block_words(uint32_t threads) {  // LDS
@@ -1173,7 +1175,8 @@ struct Entries {
 
 // one wave (or L = 16 lanes of it), one row: the teacher's entries against the student's row.  o = sums outside S, a bitmap.
 template <class T, int L, bool GRAD>
-__device__ __forceinline__ RowGrad row_loss(const DistillArgs& a, uint64_t row, const Entries& en, const uint32_t* S, uint32_t lane, const ExpSum& o) {
+__device__ __forceinline__ RowGrad row_loss(const DistillArgs& a, uint64_t row, const Entries& en, const uint32_t* S, uint32_t lane,
+                                            const ExpSum& o) {
   // the student's scale is the fp32 one of the sums outside S, for all its classes: p stays a softmax, of a temperature off by 2^-25
   const double inv_T = a.inv_T, x_scale = (double)a.scale;
   constexpr double kLn2 = 0.69314718055994530942;
@@ -1452,7 +1455,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void distill_kernel(const Dist
   }
 }
 
-// up to 32 classes: a thread per row, rows staged in LDS and their gradients collected there in fp32.  1 M x 10 fp32, k = 4: 46 us, 1150
+// up to 32 classes: a thread per row, rows staged in LDS and their gradients collected there in fp32.  1 M x 10 fp32, k = 4: 47 us, 1150
 // vector instructions per wave of 64 rows (30 us' worth of issue): the 64-bit numbers of the rows bound it, not the 120 MB.  KK > 0:
 // k = KK entries per row, in registers with their exponentials; KK = 0: any number, read and computed again where they are needed.
 // (Up to KK = 5, 124 registers and four waves per SIMD; without the branches on entries it is 135 and 52 -> 56 us.)
@@ -1611,7 +1614,9 @@ hipError_t adjust_typed(const AdjustArgs& a, bool class_major, hipStream_t s) {
   constexpr uint32_t N = Pack<T>::N;
   AdjustTiles t{};
   if (class_major) {
-    // without histories a tile is 256 packs of rows times all its classes; the counters of a history are 64 rows wide
+    // Without a history a tile is 256 packs of rows times 16 classes (300,000 x 100 fp32 41 us; 4 classes 42, 64 classes 73, 64 packs 43;
+    // 20,000 x 2000 71, 58, 79, 59).  The counters of a history are 64 rows times 256 classes, 64 KB (64 x 64, us: 300,000 x 100 with 13
+    // entries a row 205 -> 274, 100,000 x 300 with 40 454 -> 262, 20,000 x 2000 with 200 382 -> 338).
     t.rows = a.history ? 64u : 256u * N;
     t.classes = a.K < (a.history ? 256u : 16u) ? a.K : (a.history ? 256u : 16u);
     t.class_tiles = (a.K + t.classes - 1) / t.classes;
@@ -1621,8 +1626,10 @@ hipError_t adjust_typed(const AdjustArgs& a, bool class_major, hipStream_t s) {
   }
   const uint64_t row_packs = (a.K + N - 1) / N;
   // 512 packs per tile, 256 if that leaves too few tiles for the chip (64 x 128000 bf16, 100 / 8192 entries of history: 14 / 21 us, with
-  // 1024 packs 17 / 24).  Every tile of a row reads the row's whole history: from 6000 entries a row on, 1024 threads share that and
-  // 1024 packs (32 x 50257 fp32 with 50,000 entries a row: 21 us, with 256 threads 27).
+  // 1024 packs 17 / 24; 256 packs with 100 / 2000 entries 14.7 / 15.8, 512 packs 13.2 / 14.9; below 2^17 packs both are the call's 12 us).
+  // Every tile of a row reads the row's whole history: from 6000 entries a row on, 1024 threads share that and 1024 packs (32 x 50257 fp32
+  // with 15,000 / 50,000 entries a row: 14.0 / 20.8 us, with 256 threads 14.9 / 34.2; 64 x 128000 bf16 with 6000 / 15,000: 26.7 / 28.9,
+  // 19.5 / 27.3).
   const bool small = a.n * row_packs < (1u << 17), many = a.history && a.history_len / a.n > 6000u;
   const uint32_t budget = many ? 1024u : small ? 256u : 512u;
   const uint32_t ppr = (uint32_t)(row_packs < budget ? row_packs : budget);
@@ -1690,17 +1697,28 @@ hipError_t top_lanes(const TopArgs& a, uint32_t p, hipStream_t s) {
 template <class T>
 hipError_t top_typed(const TopArgs& a, bool class_major, hipStream_t s) {
   constexpr uint32_t N = Pack<T>::N;
+  // counted ranks against 16 lanes or a wave per row, us: 1 M x 16, k = 9 42 / 218, 1 M x 32, k = 17 152 / 1274 (4096 x 32 15 / 11)
   if (a.K <= 32u && a.k > 8u) return class_major ? top_rank<T, true>(a, s) : top_rank<T, false>(a, s);
-  // a thread per row reads class-major rows as they lie; with many classes it takes many rows to fill the chip
+  // A thread per row reads class-major rows as they lie; with many classes it takes many rows to fill the chip.  Against 16 lanes or a wave,
+  // us, k = 4, class-major fp32: 32,768 x 40 / 300 10.4 / 52 against 10.7 / 27, 65,536 x 40 / 300 / 1000 10.6 / 51 / 152 against 12.6 / 42 /
+  // 125, 131,072 x 300 59 against 73, 300,000 x 100 34 against 58.  Row-major: 32,768 x 64 17.9 against 10.6, 65,536 x 40 11.7 against 11.7,
+  // 1 M x 40 81 against 126, 1 M x 64 fp32 / bf16 164 / 87 against 124 / 161, 1 M x 10 (k = 3) 18 against 104.
   if (class_major && a.k <= 8u && (a.K <= 32u || a.n >= 65536u)) return top_thread<T, true>(a, s);
   if (!class_major && a.k <= 8u && (a.K <= 32u || (a.K <= 64u && a.n >= 65536u))) return top_thread<T, false>(a, s);
   if (class_major && a.K > kTopMaxClassMajor) return hipErrorInvalidValue;
-  // 16 lanes per row take out the best k times, 5 instructions per score and 40 each: against about 600 per row for a whole wave
+  // 16 lanes per row take out the best k times, 5 instructions per score and 40 each: against about 600 per row for a whole wave.  (us, fp32,
+  // 16 lanes / wave: 75,000 x 200, k = 8 / 12 / 16 38 / 51 / 65 against 52 / 53 / 53, 30,000 x 500, k = 8 / 12 / 16 32 / 42 / 52 against 27 /
+  // 28 / 29, 150,000 x 100, k = 16 75 against 94, 16,384 x 500, k = 4 14 against 17; 4096 rows and fewer are the call's 11 us either way.)
   const uint32_t packs = (a.K + N - 1) / N, p = packs <= 16u ? 1u : packs <= 32u ? 2u : packs <= 64u ? 4u : 8u;
   if (a.n >= 4096u && a.k <= 16u && packs <= 512u / N && a.k * (5u * p * N + 40u) <= 2400u)
     return class_major ? top_lanes<T, true>(a, p, s) : top_lanes<T, false>(a, p, s);
   if (class_major) return top_wave<T, true>(a, s);
+  // a wave against a block of 256, us: 16,384 x 1000 fp32, k = 20 / 200 24 / 106 against 54 / 248, 16,384 x 2048 39 / 146 against 56 / 274,
+  // 16 x 2048, k = 200 29 against 19
   if (a.K <= 2048u) return top_wave<T, false>(a, s);
+  // 256 threads against 512 (1024 for up to 256 rows), us, k = 50: 4000 x 16,000 fp32 / bf16 60 / 35 against 67 / 47, 4000 x 24,000 80 / 47
+  // against 87 / 63, 1000 x 50,000 41 / 24 against 43 / 27, 200 x 50,000 17 / 13 against 14 / 12.  512 against 1024, bf16: 256 x 128,000 18
+  // either way, 64 x 128,000 15.7 / 14.7, 384 x 50,257 16 / 21, 1024 x 128,000 58 / 66
   if (a.K <= 16384u) return top_block<T, 256>(a, s);
   return a.n > 256u ? top_block<T, 512>(a, s) : top_block<T, 1024>(a, s);
 }
@@ -1714,6 +1732,8 @@ hipError_t distill_rows(const DistillArgs& a, hipStream_t s) {
 template <class T, bool GRAD>
 hipError_t distill_typed(const DistillArgs& a, hipStream_t s) {
   constexpr uint32_t per_word = 4 / sizeof(T);
+  // a thread per row against 16 lanes, us, gradient: 1 M x 10 fp32, k = 2 / 8 37 / 105 against 285 / 305, 1 M x 32 128 / 213 against 308 / 334
+  // (4096 x 32, k = 8 19 against 12); entries in registers against reading them again, 1 M x 10, k = 1 .. 5: 33 37 41 44 47 against 39 45 51 57 63
   if (a.K <= 32u) {
     const uint32_t pitch = (((a.K + per_word - 1) / per_word) | 1u) * per_word;
     const uint32_t lds = 256u * (pitch * (uint32_t)sizeof(T) + (GRAD ? (a.K | 1u) * 4u : 0u));
@@ -1730,7 +1750,8 @@ hipError_t distill_typed(const DistillArgs& a, hipStream_t s) {
   const uint32_t packs = (a.K + Pack<T>::N - 1) / Pack<T>::N;
   // Short rows: what a row does once (its 64-bit numbers, its reductions) outweighs its scores, so four of them share a wave -- where there
   // are rows enough to fill the chip that way.  (100 M scores, us, 64 -> 16 threads per row: loss + gradient of 200 bf16 classes 922 -> 333,
-  // 500 fp32 386 -> 271, 1500 bf16 212 -> 171; 1000 fp32 239 -> 258.)
+  // 500 fp32 386 -> 271, 1500 bf16 212 -> 171; 1000 fp32 239 -> 258.  8192 x 400 fp32 18 -> 14, 4096 x 1000 15 -> 18.5, fewer rows are the
+  // call's 12.5 either way; 50,000 x 300, k = 16 / 64 77 / 108 -> 43 / 105.)
   if (a.n >= 4096u && a.k <= 64u && packs <= 256u) {
     if (packs <= 16u) return distill_rows<T, 16, 1, GRAD>(a, s);
     if (packs <= 32u) return distill_rows<T, 16, 2, GRAD>(a, s);
@@ -1738,6 +1759,8 @@ hipError_t distill_typed(const DistillArgs& a, hipStream_t s) {
     if (packs <= 128u) return distill_rows<T, 16, 8, GRAD>(a, s);
     return distill_rows<T, 16, 16, GRAD>(a, s);
   }
+  // a wave against a block of 256, gradient, us: 60,000 rows of 64 / 256 / 512 packs fp32 132 / 179 / 272 against 381 / 417 / 445, 600 rows of
+  // 512 packs 15.3 against 12.8
   if (packs <= 64u) return distill_rows<T, 64, 1, GRAD>(a, s);
   if (packs <= 128u) return distill_rows<T, 64, 2, GRAD>(a, s);
   if (packs <= 256u) return distill_rows<T, 64, 4, GRAD>(a, s);
@@ -1745,10 +1768,17 @@ hipError_t distill_typed(const DistillArgs& a, hipStream_t s) {
   // few rows: as many threads on each as there are.  Else enough blocks per CU that one row's ends are hidden behind the other rows'
   // packs -- for the gradient no more than keep their rows in the 256 MB cache until their second read, and in registers where a thread's
   // packs fill them.  (us with 256 / 512 / 1024 threads: loss of 2048 x 50257 fp16 51 / 54 / 72; gradient of 8192 x 128000 bf16
-  // 1123 / 951 / 1148, 2000 x 100000 fp32 457 / 402 / 400; 12200 x 16384 fp32 in registers 336, read twice 372.)
+  // 1123 / 951 / 1148, 2000 x 100000 fp32 457 / 402 / 400; 200 M bf16 scores with 512 / 1024 threads, rows of 5000 packs 213 / 333, of 16,000
+  // 223 / 245, of 20,000 221 / 221.  1024 threads / fewer for few rows: gradient of 256 x 20,000 bf16 13.7 / 16.7, of 512 24.3 / 20.1, loss of
+  // 256 x 50,257 10.9 / 12.5, of 512 17.9 / 14.3.)
   if (a.n <= 512u) return distill_rows<T, 1024, 0, GRAD>(a, s);
+  // four packs a thread in registers against reading twice, us: 20,000 rows of 600 / 1000 packs, gradient fp32 162 / 179 against 187 / 228, bf16
+  // 226 / 251 against 212 / 261, loss fp32 66 / 70 against 72 / 88
   if (packs <= 1024u) return distill_rows<T, 256, 4, GRAD>(a, s);
   if constexpr (GRAD) {
+    // Reading twice against 16 packs a thread in registers (136 of them: three waves per SIMD, however many of the packs are there), us: 12,000
+    // rows of 1100 / 2000 / 2900 / 3300 / 4000 packs fp32 115 / 192 / 268 / 290 / 360 against 193 / 221 / 252 / 268 / 304, of 2900 bf16 276
+    // against 301; 1000 rows of 4000, which the cache holds, 33 against 38.
     if (packs <= 3000u) return distill_rows<T, 256, 0, GRAD>(a, s);
     if (packs <= 4096u) return distill_rows<T, 256, 16, GRAD>(a, s);
     return packs <= 16384u ? distill_rows<T, 512, 0, GRAD>(a, s) : distill_rows<T, 1024, 0, GRAD>(a, s);
